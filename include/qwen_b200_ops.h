@@ -85,6 +85,92 @@ int qwen_b200_prefill_approx_exp(const float* x, float* y, long long n, void* st
  * x, y [n] fp32 device memory. */
 int qwen_b200_exact_expf(const float* x, float* y, long long n, void* stream);
 
+/* Element types of the operators below. Whatever the type, they compute in fp32 and round results once. */
+enum { QWEN_B200_F32 = 0, QWEN_B200_F16 = 1, QWEN_B200_BF16 = 2 };
+
+/* An 8-bit KV cache of one layer, in buffers of the caller (device memory): blocks of 64 tokens, head dimension
+ * 128, int8 codes, one fp32 scale per block and kv head; a cached value is code * scale. No counterpart in the
+ * reference, whose caches are fp32 (hls/common/llm_memory_layout.h).
+ *   k_codes, v_codes    [n_blocks][n_kv_heads][64][128] int8 (16-byte aligned)
+ *   k_scales, v_scales  [n_blocks][n_kv_heads] fp32
+ *   block_table         [n_seqs][max_blocks] int32: token t of sequence s is slot t % 64 of block
+ *                       block_table[s][t / 64]; entries behind a sequence's last block are not read
+ * Blocks need no initialisation. Indexes that live on the device are checked there: a kernel that meets one outside
+ * of its buffers skips the access and sets bit 1 of qwen_b200_kernel_error(); values of such a place read as NaN. */
+typedef struct qwen_b200_kv8_cache {
+  signed char* k_codes;
+  signed char* v_codes;
+  float* k_scales;
+  float* v_scales;
+  int n_blocks;
+  int n_kv_heads;
+  const int* block_table;
+  int n_seqs;
+  int max_blocks;
+} qwen_b200_kv8_cache;
+
+/* Write K and V rows into the cache (each row: n_kv_heads x 128 values, row_stride elements apart, so that rows may
+ * lie inside q|k|v rows). Segment i appends rows offsets[i] .. offsets[i + 1] - 1 to sequence seqs[i], which holds
+ * starts[i] tokens already; offsets [n_segments + 1] ascend from 0, equal ones make an empty segment, and rows from
+ * offsets[n_segments] to n_rows (a padded batch) are ignored. Per kv head, for K and for V:
+ *   a block that the call opens (its first new slot is slot 0) gets scale = max|x| * fl(1 / 127), at least 2^-126 (0
+ *   if every value is 0); a block with earlier tokens keeps its scale, doubled as often as needed to reach that value,
+ *   and the codes of its earlier tokens are halved as often; code = clamp(rint(x / scale), -127, 127), ties to even.
+ * A value written with its whole block is off by at most scale / 2, one that was halved later by less than scale.
+ * Appending again from an earlier position (a dropped draft) overwrites. A NaN or an infinity makes its block's scale
+ * NaN: the block reads as NaN until it is opened again.
+ * A block shared by several sequences must not be written, and a call must not name a sequence twice (the values of
+ * such blocks would be undefined, with no access out of bounds).
+ *   k, v                  [n_rows] rows of `dtype` (16-byte aligned; row_stride a multiple of 16 bytes)
+ *   seqs, starts, offsets [n_segments], [n_segments], [n_segments + 1] int32 (device memory) */
+int qwen_b200_kv8_append(const qwen_b200_kv8_cache* cache, const void* k, const void* v, int dtype,
+                         long long row_stride, long long n_rows, const int* seqs, const int* starts,
+                         const int* offsets, int n_segments, void* stream);
+
+/* Read cached rows back: segment i writes tokens starts[i] .. of sequence seqs[i] to rows offsets[i] ..
+ * offsets[i + 1] - 1 of k and v, as code * scale rounded to `dtype`. Arguments as above; rows from
+ * offsets[n_segments] on are left as they are, and a sequence may be named more than once. */
+int qwen_b200_kv8_read(const qwen_b200_kv8_cache* cache, void* k, void* v, int dtype, long long row_stride,
+                       long long n_rows, const int* seqs, const int* starts, const int* offsets, int n_segments,
+                       void* stream);
+
+/* Decode attention over the 8-bit cache, one query row per new token (replaces the context of
+ * hls/decode_only/qwen_decode_attention_kernel.cpp:113-162 for a cache in this form). Row r of sequence
+ * row_seqs[r] attends to the sequence's first row_lens[r] tokens (its own included: append first); drafted tokens of
+ * one sequence are rows with lengths that rise by one. Query head h reads kv head h / (n_q_heads / n_kv_heads).
+ *   s_j = scale * (q . k_j),  out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j)
+ * row_lens[r] == 0: out is 0 and lse -infinity. row_seqs[r] < 0 (a padded row): out and lse are left as they are.
+ *   q, out     [n_rows] rows of n_q_heads x 128 values of `dtype` (16-byte aligned, strides in elements, multiples
+ *              of 16 bytes); out must not overlap q
+ *   row_seqs, row_lens  [n_rows] int32 (device memory)
+ *   workspace  at least qwen_b200_kv8_attention_workspace(n_rows, n_q_heads, n_kv_heads) bytes of device memory
+ *              (16-byte aligned, any contents); calls that overlap on the GPU need one each
+ *   lse        [n_rows][n_q_heads] fp32, or NULL */
+int qwen_b200_kv8_attention(const qwen_b200_kv8_cache* cache, const void* q, long long q_stride, void* out,
+                            long long out_stride, int dtype, int n_rows, int n_q_heads, const int* row_seqs,
+                            const int* row_lens, float scale, void* workspace, long long workspace_bytes, float* lse,
+                            void* stream);
+/* Bytes of that workspace, -1 for an argument out of range. */
+long long qwen_b200_kv8_attention_workspace(int n_rows, int n_q_heads, int n_kv_heads);
+
+/* Sample one token per row from its logits and a given uniform number (the reference only takes the argmax,
+ * verification/real_host_top_backend.py:138-146). With the row's tokens sorted by logit (ties: lowest index first),
+ * w_i = exp((logit_i - max) / temperature):
+ *   top_k > 0  keeps the first top_k;
+ *   top_p < 1  keeps the fewest of those, at least one, whose sum of w reaches top_p of their whole sum;
+ *   min_p > 0  keeps those of w >= min_p (the first one in any case);
+ * the token is the first whose running sum of w exceeds uniform * (sum of the kept w), the last one kept if none does.
+ * temperature below 2^-126 (0 included) or NaN: the first token, with probability 1. Logits of -infinity or NaN are
+ * never taken; a row without any other gives token -1, probability 0. +infinity outweighs every finite logit.
+ *   logits      [rows][vocab] of `dtype`, rows row_stride elements apart; 1 <= vocab <= 262144
+ *   temperature, top_k, top_p, min_p  [rows] fp32 / int32, or NULL (1, off, off, off)
+ *   uniforms    [rows] fp32 in [0, 1)
+ *   tokens      [rows] int32;  probs  [rows] fp32: the probability that the token had among the kept ones, or NULL
+ * All device memory. The result does not depend on the order in which anything is summed on the GPU. */
+int qwen_b200_sample(const void* logits, int dtype, int rows, int vocab, long long row_stride, const float* temperature,
+                     const int* top_k, const float* top_p, const float* min_p, const float* uniforms, int* tokens,
+                     float* probs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

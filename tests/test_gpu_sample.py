@@ -1,0 +1,254 @@
+"""GPU tests of token sampling (include/qwen_b200_ops.h) against the plain float64 model in kv8_model.py. Uniform
+numbers and top_p values are put in the middle between two borders, at least 1e-6 of the whole from either, where the
+kernel's weights (each within 2^-20 of the exact one, so their sums too) cannot change the answer."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import kv8_model as km
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+@pytest.fixture(autouse=True)
+def _device(built_libs, gpu_available):
+    if not gpu_available:
+        pytest.fail("no CUDA device: the -m gpu suite must run on a B200")
+
+
+def run(logits, u, dtype="f32", temperature=None, top_k=None, top_p=None, min_p=None, vocab=None, probs=True):
+    """logits [rows][>= vocab] torch tensor of its type on the CPU; the settings lists or None."""
+    import torch
+    from work_llm_accelerator_b200 import host
+
+    x = logits.cuda()
+    n = x.shape[0]
+    vocab = x.shape[1] if vocab is None else vocab
+    f = lambda v, t: None if v is None else torch.tensor(v, dtype=t).cuda()  # noqa: E731
+    t, k, p, m = f(temperature, torch.float32), f(top_k, torch.int32), f(top_p, torch.float32), f(min_p, torch.float32)
+    u = f(u, torch.float32)
+    tokens = torch.full((n,), -9, dtype=torch.int32).cuda()
+    out = torch.full((n,), -9.0).cuda()
+    ptr = lambda v: 0 if v is None else v.data_ptr()  # noqa: E731
+    host.sample(x.data_ptr(), TYPES[dtype], n, vocab, x.stride(0), ptr(t), ptr(k), ptr(p), ptr(m), u.data_ptr(),
+                tokens.data_ptr(), out.data_ptr() if probs else 0, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return tokens.cpu().numpy(), out.cpu().numpy()
+
+
+def middle(w, r):
+    """A uniform number in the middle of the interval of one of the larger weights, and that weight's place."""
+    p = w / w.sum()
+    at = int(r.choice(np.nonzero(p >= min(1e-5, p.max()))[0]))
+    return float((np.cumsum(p)[at] - p[at] / 2)), at
+
+
+def check(rows, dtype, seed, **settings):
+    """Every row: filters on, u in the middle of a kept token's interval."""
+    import torch
+
+    r = np.random.RandomState(seed)
+    x = rows.float().numpy()
+    n = len(x)
+    us, want, want_p = [], [], []
+    for i in range(n):
+        f = {k: v[i] for k, v in settings.items() if v is not None}
+        if "temperature" in f:
+            f["temperature"] = np.float32(f["temperature"])
+        ids, w = km.kept(x[i], **{k: (float(np.float32(v)) if k != "top_k" else v) for k, v in f.items()})
+        if len(ids) == 0:
+            us.append(0.5), want.append(-1), want_p.append(0.0)
+            continue
+        u, at = middle(w, r)
+        us.append(u), want.append(ids[at]), want_p.append(w[at] / w.sum())
+    got, p = run(rows, us, dtype, **settings)
+    np.testing.assert_array_equal(got, want)
+    np.testing.assert_allclose(p, want_p, rtol=2.0**-18, atol=0)  # 2^-20 of a weight and of their sum, rounding
+
+
+def gaussian(rows, vocab, dtype, seed, size=1.7, peak=6.0):
+    import torch
+
+    g = torch.Generator().manual_seed(seed)
+    x = size * torch.randn(rows, vocab, generator=g)
+    x[:, torch.randperm(vocab, generator=g)[: min(vocab, 30)]] += peak * torch.rand(rows, min(vocab, 30), generator=g)
+    return x.to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype])
+
+
+def safe_top_p(x, temperature, top_k, near):
+    """Per row a top_p near `near` that lies in the middle of a token's share."""
+    out = []
+    for i in range(len(x)):
+        _, w = km.kept(x[i].float().numpy(), float(np.float32(temperature[i])) if temperature else 1.0, top_k[i] if top_k else 0)
+        c = np.cumsum(w) / w.sum()
+        p = w / w.sum()
+        ok = np.nonzero(p >= min(4e-6, p.max()))[0]
+        at = ok[np.argmin(np.abs(c[ok] - near))]
+        out.append(float(c[at] - p[at] / 2))
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 2, 31, 1000, 4097, 50257, 151936, 262144])
+def test_plain_sampling(dtype, vocab):
+    check(gaussian(3, vocab, dtype, vocab), dtype, vocab, temperature=[0.7, 1.0, 1.3])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [7, 1000, 151936])
+@pytest.mark.parametrize("k", [1, 2, 50, 900, 70000])
+def test_top_k(dtype, vocab, k):
+    check(gaussian(2, vocab, dtype, k), dtype, k, temperature=[0.8, 1.5], top_k=[k, max(1, k // 2)])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("near", [0.01, 0.5, 0.9, 0.97])
+@pytest.mark.parametrize("vocab,size,peak", [(1000, 1.7, 6.0), (151936, 1.7, 6.0), (151936, 1.7, 12.0)])
+def test_top_p_alone_and_after_top_k(dtype, near, vocab, size, peak):
+    x = gaussian(4, vocab, dtype, int(near * 100), size, peak)
+    t, k = [0.6, 1.0, 1.0, 0.9], [0, 0, 40, 300]
+    check(x, dtype, 1, temperature=t, top_k=k, top_p=safe_top_p(x, t, k, near))
+
+
+@pytest.mark.parametrize("min_p", [1e-6, 0.013, 0.3, 1.0, 2.0])
+def test_min_p(min_p):
+    """The border is compared in 64 bits; rows where a weight lies within 2^-40 of it do not occur here."""
+    x = gaussian(3, 20000, "f32", 5)
+    check(x, "f32", 2, temperature=[0.9, 1.0, 1.1], min_p=[min_p] * 3)
+
+
+def test_all_filters_with_rows_of_their_own():
+    x = gaussian(24, 151936, "bf16", 8)
+    r = np.random.RandomState(1)
+    t = [0.0 if i % 7 == 3 else float(0.4 + r.rand()) for i in range(24)]
+    k = [int(v) for v in r.randint(0, 80, 24)]
+    p = safe_top_p(x, [v or 1.0 for v in t], k, 0.9)
+    p = [1.0 if i % 5 == 0 else v for i, v in enumerate(p)]
+    check(x, "bf16", 3, temperature=t, top_k=k, top_p=p, min_p=[0.0 if i % 3 else 0.02 for i in range(24)])
+
+
+@pytest.mark.parametrize("vocab", [1, 5, 8193, 151936])
+@pytest.mark.parametrize("k", [0, 3, 2000, 100000])
+def test_ties_go_to_the_lowest_index(vocab, k):
+    """Every logit equal: token j's interval is the j-th. Zeros of both signs tie."""
+    import torch
+
+    x = torch.zeros(2, vocab)
+    x[1, ::2] = -0.0
+    n = min(k, vocab) if k else vocab
+    js = [0, n - 1]
+    got, p = run(x, [(j + 0.5) / n for j in js], top_k=[k, k])
+    assert list(got) == js
+    np.testing.assert_allclose(p, 1.0 / n, rtol=2.0**-18)
+    # half of the mass: top_p in the middle of the share of token m
+    m = n // 2
+    got, p = run(x, [(m + 0.5) / (m + 1)] * 2, top_k=[k, k], top_p=[(m + 0.5) / n] * 2)
+    assert list(got) == [m, m]
+    np.testing.assert_allclose(p, 1.0 / (m + 1), rtol=2.0**-18)
+
+
+def test_two_levels_of_ties():
+    """70000 tokens tie at the border of the kept set."""
+    import torch
+
+    x = torch.full((1, 151936), -1.0)
+    x[0, 50000:120000] = 0.25
+    x[0, [149000, 3]] = 0.5
+    ids, w = km.kept(x[0].numpy(), 1.0, 30002)
+    for at in (0, 1, 2, 3, 15000, 30001):
+        p = w / w.sum()
+        got, _ = run(x, [float(np.cumsum(p)[at] - p[at] / 2)], top_k=[30002])
+        assert got[0] == ids[at], at
+
+
+@pytest.mark.parametrize("spread", [1e-6, 1e-3, 0.05])
+def test_crowded_logits(spread):
+    """All logits within a narrow band: thousands share what a coarse view would call one value."""
+    x = gaussian(2, 151936, "f32", 4, size=spread, peak=0.0)
+    check(x, "f32", 5, top_k=[100, 77777])
+    check(x, "f32", 6, temperature=[1.0, 30.0], top_p=safe_top_p(x, [1.0, 30.0], None, 0.4))
+
+
+def test_masked_rows_and_infinities():
+    import torch
+
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[-inf, -inf, -inf, -inf], [nan, nan, -inf, nan], [-inf, 2.0, nan, 2.0], [1.0, inf, 3.0, inf],
+                      [-inf, -3e38, 3e38, 3e38], [3.0, 1.0, -inf, 3.0]])
+    for t in (0.0, 0.5, 1.0):
+        got, p = run(x, [0.6] * 6, temperature=[t] * 6, top_k=[3] * 6, top_p=[0.99] * 6, min_p=[0.1] * 6)
+        assert list(got) == ([-1, -1, 1, 1, 2, 0] if t == 0 else [-1, -1, 3, 3, 3, 3])
+        # the last row keeps its third token where e^(-2 / t) is at least 0.1
+        last = 0.5 if t == 0.5 else 1 / (2 + np.exp(-2.0))
+        np.testing.assert_allclose(p, [0, 0, 1, 1, 1, 1] if t == 0 else [0, 0, 0.5, 0.5, 0.5, last], rtol=2.0**-18)
+
+
+def test_a_mask_of_the_lowest_value():
+    """Banned tokens as the type's lowest value instead of -infinity: weight 0 next to any other, equal among themselves."""
+    import torch
+
+    low = torch.finfo(torch.float32).min
+    x = torch.full((2, 5000), low)
+    x[0, 4321] = 1.0
+    got, p = run(x, [0.9999, (1234 + 0.5) / 5000])
+    assert list(got) == [4321, 1234] and p[0] == 1.0
+
+
+@pytest.mark.parametrize("t", [float("nan"), -1.0, 1e-40, 2.0**-126, 1e-3, 1e30, float("inf")])
+def test_extreme_temperatures(t):
+    import torch
+
+    x = torch.tensor([[0.5, 2.0, 1.0, 2.0]])
+    if not t >= 2.0**-126:
+        want = [(0.7, 1, 1.0)]
+    elif t < 1:
+        want = [(0.25, 1, 0.5), (0.75, 3, 0.5)]
+    else:
+        want = [(0.125, 1, 0.25), (0.375, 3, 0.25), (0.625, 2, 0.25), (0.875, 0, 0.25)]
+    for u, token, prob in want:
+        got, p = run(x, [u], temperature=[t])
+        assert got[0] == token
+        np.testing.assert_allclose(p, prob, rtol=2.0**-18)
+
+
+def test_settings_at_their_borders():
+    import torch
+
+    x = torch.tensor([[1.0, 3.0, 2.0]])
+    for kw in ({"top_p": [0.0]}, {"top_p": [-1.0]}, {"top_k": [1]}, {"min_p": [1.0]}, {"min_p": [5.0]}):
+        for u in (0.0, 0.999):
+            assert run(x, [u], **kw)[0][0] == 1, kw
+    for kw in ({"top_p": [1.0]}, {"top_p": [2.0]}, {"top_p": [float("nan")]}, {"top_k": [0]}, {"top_k": [-3]}, {"top_k": [99]},
+               {"min_p": [0.0]}, {"min_p": [-1.0]}, {"min_p": [float("nan")]}):
+        assert run(x, [0.0], **kw)[0][0] == 1 and run(x, [0.999], **kw)[0][0] == 0, kw
+    # uniform numbers outside of [0, 1): the first and the last kept token
+    for u, token in ((-1.0, 1), (float("nan"), 1), (1.0, 0), (7.0, 0)):
+        assert run(x, [u])[0][0] == token
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab,stride", [(1001, 1001), (1000, 1003), (151935, 151936), (50257, 50300)])
+def test_strides_and_alignment(dtype, vocab, stride):
+    """Rows that start at any element; what lies between them must not be read as logits."""
+    import torch
+
+    x = gaussian(3, vocab, dtype, 9)
+    wide = torch.full((3, stride), 60000.0).to(x.dtype)
+    wide[:, :vocab] = x
+    us = [0.1, 0.5, 0.8]
+    want, wp = run(x, us, dtype, top_k=[50] * 3)
+    got, p = run(wide, us, dtype, top_k=[50] * 3, vocab=vocab)
+    np.testing.assert_array_equal(got, want)
+    np.testing.assert_array_equal(p, wp)
+
+
+def test_many_rows_repeat_exactly_and_without_probs():
+    x = gaussian(400, 5000, "f32", 12)
+    us = list(np.linspace(0, 0.999, 400))
+    a, p = run(x, us, top_p=[0.9] * 400)
+    b, q = run(x, us, top_p=[0.9] * 400)
+    c, none = run(x, us, top_p=[0.9] * 400, probs=False)
+    assert (a == b).all() and (p == q).all() and (a == c).all() and (none == -9).all()

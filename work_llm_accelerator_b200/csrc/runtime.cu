@@ -22,6 +22,7 @@
 #include "layer0_ref.h"
 #include "decode_bs1.h"
 #include "decode_stack.h"
+#include "kv8.h"
 #include "qgemm.h"
 #include "lmhead.h"
 #include "tgemm.h"
@@ -592,7 +593,8 @@ unsigned qwen_b200_kernel_error(int reset) {
          qb::stack::decode_stack_kernel_error(reset != 0) | qb::bs1::decode_bs1_kernel_error(reset != 0) |
          qb::tgemm_kernel_error(reset != 0) |
          qb::lm_head_kernel_error(reset != 0) | qb::attn_tc_kernel_error(reset != 0) |
-         qb::decode_attn_kernel_error(reset != 0);
+         qb::decode_attn_kernel_error(reset != 0) | qb::kv8::kernel_error(reset != 0) |
+         qb::kv8::attention_kernel_error(reset != 0);
 }
 
 int qwen_b200_device_count(void) {

@@ -12,6 +12,7 @@ namespace qb {
 static __device__ unsigned g_kernel_error;
 
 constexpr unsigned kErrMbarTimeout = 1u;
+constexpr unsigned kErrBadIndex = 2u;  // a device-side index outside of its buffer; the access was skipped
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

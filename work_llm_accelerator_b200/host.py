@@ -43,6 +43,14 @@ class NativeLibraryMissing(RuntimeError):
     pass
 
 
+class _Kv8Struct(ctypes.Structure):
+    """qwen_b200_kv8_cache (include/qwen_b200_ops.h)."""
+
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("n_blocks", ctypes.c_int), ("n_kv_heads", ctypes.c_int),
+                ("block_table", ctypes.c_void_p), ("n_seqs", ctypes.c_int), ("max_blocks", ctypes.c_int)]
+
+
 def _open(path: Path) -> ctypes.CDLL:
     if not path.exists():
         raise NativeLibraryMissing(
@@ -80,6 +88,17 @@ def core_lib() -> ctypes.CDLL:
         lib.qwen_b200_prefill_approx_exp.restype = ctypes.c_int
         lib.qwen_b200_exact_expf.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]
         lib.qwen_b200_exact_expf.restype = ctypes.c_int
+        vp, i, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+        for name in ("qwen_b200_kv8_append", "qwen_b200_kv8_read"):
+            getattr(lib, name).argtypes = [ctypes.POINTER(_Kv8Struct), vp, vp, i, i64, i64, vp, vp, vp, i, vp]
+            getattr(lib, name).restype = i
+        lib.qwen_b200_kv8_attention.argtypes = [ctypes.POINTER(_Kv8Struct), vp, i64, vp, i64, i, i, i, vp, vp,
+                                                ctypes.c_float, vp, i64, vp, vp]
+        lib.qwen_b200_kv8_attention.restype = i
+        lib.qwen_b200_kv8_attention_workspace.argtypes = [i, i, i]
+        lib.qwen_b200_kv8_attention_workspace.restype = i64
+        lib.qwen_b200_sample.argtypes = [vp, i, i, i, i64] + [vp] * 8
+        lib.qwen_b200_sample.restype = i
         lib.qwen_b200_kernel_error.argtypes = [ctypes.c_int]
         lib.qwen_b200_kernel_error.restype = ctypes.c_uint
         _core = lib
@@ -508,3 +527,71 @@ def w8_digit_planes(codes_ptr: int, rows: int, k: int, x_ptr: int, n_tokens: int
     st = core_lib().qwen_b200_w8_digit_planes(codes_ptr, rows, k, x_ptr, n_tokens, acc_ptr, step_ptr, stream or None)
     if st != 0:
         raise EngineError(f"qwen_b200_w8_digit_planes failed with status {st}: {last_error()}")
+
+
+# ---------------------------------------------------------------------------------------------------
+# 8-bit KV cache and sampling (include/qwen_b200_ops.h): raw device addresses, enqueued on `stream`
+# ---------------------------------------------------------------------------------------------------
+F32, F16, BF16 = 0, 1, 2  # element types of the operators below
+KV8_BLOCK = 64  # tokens that share one scale per kv head
+
+
+class Kv8Cache:
+    """Describes an 8-bit KV cache of one layer in the caller's device buffers: int8 codes
+    [n_blocks][n_kv_heads][64][128], fp32 scales [n_blocks][n_kv_heads], int32 block table [n_seqs][max_blocks]."""
+
+    def __init__(self, k_codes_ptr: int, v_codes_ptr: int, k_scales_ptr: int, v_scales_ptr: int, n_blocks: int,
+                 n_kv_heads: int, block_table_ptr: int, n_seqs: int, max_blocks: int):
+        self.struct = _Kv8Struct(k_codes_ptr, v_codes_ptr, k_scales_ptr, v_scales_ptr, n_blocks, n_kv_heads,
+                                 block_table_ptr, n_seqs, max_blocks)
+        self.ref = ctypes.byref(self.struct)
+
+
+def kv8_append(cache: Kv8Cache, k_ptr: int, v_ptr: int, dtype: int, row_stride: int, n_rows: int, seqs_ptr: int,
+               starts_ptr: int, offsets_ptr: int, n_segments: int, stream: int = 0) -> None:
+    """Quantise rows into the cache: segment i appends rows offsets[i]..offsets[i+1]-1 to sequence seqs[i], which
+    holds starts[i] tokens."""
+    st = core_lib().qwen_b200_kv8_append(cache.ref, k_ptr, v_ptr, dtype, row_stride, n_rows, seqs_ptr, starts_ptr,
+                                         offsets_ptr, n_segments, stream or None)
+    if st != 0:
+        raise EngineError(f"qwen_b200_kv8_append failed with status {st}: {last_error()}")
+
+
+def kv8_read(cache: Kv8Cache, k_ptr: int, v_ptr: int, dtype: int, row_stride: int, n_rows: int, seqs_ptr: int,
+             starts_ptr: int, offsets_ptr: int, n_segments: int, stream: int = 0) -> None:
+    """Read cached rows back as code * scale: tokens starts[i].. of sequence seqs[i] to rows offsets[i].."""
+    st = core_lib().qwen_b200_kv8_read(cache.ref, k_ptr, v_ptr, dtype, row_stride, n_rows, seqs_ptr, starts_ptr,
+                                       offsets_ptr, n_segments, stream or None)
+    if st != 0:
+        raise EngineError(f"qwen_b200_kv8_read failed with status {st}: {last_error()}")
+
+
+def kv8_attention_workspace(n_rows: int, n_q_heads: int, n_kv_heads: int) -> int:
+    """Bytes of device memory that kv8_attention needs as its workspace."""
+    n = core_lib().qwen_b200_kv8_attention_workspace(n_rows, n_q_heads, n_kv_heads)
+    if n < 0:
+        raise EngineError(f"qwen_b200_kv8_attention_workspace: {last_error()}")
+    return n
+
+
+def kv8_attention(cache: Kv8Cache, q_ptr: int, q_stride: int, out_ptr: int, out_stride: int, dtype: int, n_rows: int,
+                  n_q_heads: int, row_seqs_ptr: int, row_lens_ptr: int, scale: float, workspace_ptr: int,
+                  workspace_bytes: int, lse_ptr: int = 0, stream: int = 0) -> None:
+    """Decode attention over the cache: row r attends to the first row_lens[r] tokens of sequence row_seqs[r]."""
+    st = core_lib().qwen_b200_kv8_attention(cache.ref, q_ptr, q_stride, out_ptr, out_stride, dtype, n_rows, n_q_heads,
+                                            row_seqs_ptr, row_lens_ptr, scale, workspace_ptr, workspace_bytes,
+                                            lse_ptr or None, stream or None)
+    if st != 0:
+        raise EngineError(f"qwen_b200_kv8_attention failed with status {st}: {last_error()}")
+
+
+def sample(logits_ptr: int, dtype: int, rows: int, vocab: int, row_stride: int, temperature_ptr: int, top_k_ptr: int,
+           top_p_ptr: int, min_p_ptr: int, uniforms_ptr: int, tokens_ptr: int, probs_ptr: int = 0,
+           stream: int = 0) -> None:
+    """Sample one token per row with temperature, top-k, top-p and min-p (a setting's address may be 0: off) from
+    given uniform numbers."""
+    st = core_lib().qwen_b200_sample(logits_ptr, dtype, rows, vocab, row_stride, temperature_ptr or None,
+                                     top_k_ptr or None, top_p_ptr or None, min_p_ptr or None, uniforms_ptr, tokens_ptr,
+                                     probs_ptr or None, stream or None)
+    if st != 0:
+        raise EngineError(f"qwen_b200_sample failed with status {st}: {last_error()}")
