@@ -34,13 +34,13 @@ constexpr int kRows = 8;     // query heads of an item
 constexpr int kTileBytes = kTile * kHead;       // of K or V
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kPartFloats = kRows * (kHead + 2);  // sums [8][128], maxima [8], weights' sums [8]
-constexpr int kMergeThreads = 128;
+constexpr int kMergeThreads = 256;
 
 // Shared memory: the rings, then a part per warp (an item that began before the warp's run), then the stage notes.
-struct Note {
-  long long item;  // row * subs + sub
-  int valid;       // tokens of the tile that the row reaches
-  int flags;       // kFirst, kLast: the item's first and last tile; kBad: no such block
+struct __align__(16) Note {
+  int row, sub;  // the item
+  int valid;     // tokens of the tile that the row reaches
+  int flags;     // kFirst, kLast: the item's first and last tile; kBad: no such block
 };
 constexpr int kFirst = 1, kLast = 2, kBad = 4;
 constexpr int kRingBytes = kWarps * kStages * kStageBytes;
@@ -51,9 +51,9 @@ constexpr int kSmemBytes = kScalesOffset + kWarps * kStages * 2 * 4;
 static_assert(kSmemBytes + 1024 <= 227 * 1024, "shared memory of one CTA, static part included");
 
 // Workspace: parts [2 * kCtas], then which item each part belongs to. Part 2 c: an item that began before CTA c's
-// run (info = 2 * item + 1 if it ends there, else 2 * item); part 2 c + 1: one that began in it and goes on. -1: none.
+// run (info = 2 * item + 1 if it ends there, else 2 * item; item = row * subs + sub); part 2 c + 1: one that began in it and goes on. -1: none.
 constexpr size_t kInfoOffset = (size_t)2 * kCtas * kPartFloats * 4;
-constexpr size_t kWorkBytes = kInfoOffset + 2 * kCtas * sizeof(long long);
+constexpr size_t kWorkBytes = kInfoOffset + 2 * kCtas * sizeof(int);
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -66,6 +66,41 @@ __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsig
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The first product of a sum.
+__device__ __forceinline__ void mma_first(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// Pairs of fp32 numbers in one instruction.
+__device__ __forceinline__ unsigned long long pair(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(unsigned long long v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 // Two codes to two fp16 numbers: with the sign bit flipped a code is c + 128, as the low byte of 0x64xx it is the
@@ -130,23 +165,29 @@ __device__ __forceinline__ void put_lse(const Attend& a, long long row, int h, f
   if (a.lse) a.lse[row * a.q_heads + h] = m * 0.6931471805599453f + logf(l);
 }
 
+// This lane's dims of one query head, scaled by a power of two and split.
+struct Query {
+  unsigned f[8][4];  // dims 32 q4 + 4 s + {0, 1 | 2, 3} of head g, high and low
+  float scale;       // scale * log2(e) * the power of two that was taken out
+};
+
 template <int kType>
 __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
   using T = typename TypeOf<kType>::T;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long warp_sum[kWarps], start_off[kWarps], part_item[kWarps][2];
-  __shared__ int start_row[kWarps], part_ended[kWarps];
+  __shared__ long long warp_sum[kWarps];
+  __shared__ int4 start[kWarps];  // row, first tile among the row's, length, sequence
+  __shared__ int part_item[2 * kWarps], part_ended[kWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q4 = lane % 4;
   const Layout lay(c, a);
-  float* work = static_cast<float*>(a.work);
-  long long* info = reinterpret_cast<long long*>(static_cast<uint8_t*>(a.work) + kInfoOffset);
 
   // ---- the runs: tiles before each thread's rows, the whole, and where this CTA's warps begin
   const int per_thread = (a.rows + kThreads - 1) / kThreads;
   const int row0 = min(a.rows, (int)threadIdx.x * per_thread), row1 = min(a.rows, row0 + per_thread);
   long long mine = 0;
   for (int r = row0; r < row1; ++r) mine += row_tiles(c, a, r);
+  mine *= lay.subs;
   long long upto = mine;
 #pragma unroll
   for (int i = 1; i < 32; i <<= 1) {
@@ -154,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
     if (lane >= i) upto += v;
   }
   if (lane == 31) warp_sum[warp] = upto;
-  if (threadIdx.x < 2 * kWarps) part_item[threadIdx.x / 2][threadIdx.x % 2] = -1;
+  if (threadIdx.x < 2 * kWarps) part_item[threadIdx.x] = -1;
   __syncthreads();
   long long before = upto - mine, all = 0;
 #pragma unroll
@@ -162,79 +203,89 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
     if (w < warp) before += warp_sum[w];
     all += warp_sum[w];
   }
-  all *= lay.subs;
-  const long long per_cta = max((long long)kWarps, (all + gridDim.x - 1) / gridDim.x);
+  const long long per_cta = max((long long)kWarps, (all + kCtas - 1) / kCtas);
   const long long cta0 = blockIdx.x * per_cta;
-  const long long cta_n = max(0ll, min(per_cta, all - cta0));
-  const long long per_warp = (cta_n + kWarps - 1) / kWarps;
+  const int cta_n = (int)max(0ll, min(per_cta, all - cta0));  // the entry point bounds all by 2^40
+  const int per_warp = (cta_n + kWarps - 1) / kWarps;
+  if (mine > 0 && before < cta0 + cta_n && before + mine > cta0) {
+    long long pos = before;
+    for (int r = row0; r < row1; ++r) {
+      const long long n = (long long)row_tiles(c, a, r) * lay.subs;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const long long at = cta0 + w * per_warp;
-    if (mine > 0 && at >= before * lay.subs && at < (before + mine) * lay.subs) {
-      long long pos = before * lay.subs;
-      int r = row0;
-      for (; r < row1; ++r) {
-        const long long n = (long long)row_tiles(c, a, r) * lay.subs;
-        if (at < pos + n) break;
-        pos += n;
+      for (int w = 0; w < kWarps; ++w) {
+        const long long at = cta0 + w * per_warp;
+        if (at >= pos && at < pos + n) start[w] = make_int4(r, (int)(at - pos), __ldg(a.row_len + r), __ldg(a.row_seq + r));
       }
-      start_row[w] = r;
-      start_off[w] = at - pos;
+      pos += n;
     }
   }
   __syncthreads();
 
   // ---- this warp's run
-  const long long todo = max(0ll, min(per_warp, cta_n - warp * per_warp));
+  const int todo = max(0, min(per_warp, cta_n - warp * per_warp));
   uint8_t* ring = smem + warp * kStages * kStageBytes;
   float* part = reinterpret_cast<float*>(smem + kPartsOffset) + warp * kPartFloats;
   Note* notes = reinterpret_cast<Note*>(smem + kNotesOffset) + warp * kStages;
   float* scales = reinterpret_cast<float*>(smem + kScalesOffset) + warp * kStages * 2;
   if (todo > 0) {
     // the load cursor
-    int row = start_row[warp], len = __ldg(a.row_len + row), tiles = (len - 1) / kTile + 1;
-    int sub = (int)(start_off[warp] / tiles), tile = (int)(start_off[warp] % tiles);
-    const int* table = c.table + (long long)__ldg(a.row_seq + row) * c.width;
-    long long left = todo;
+    int row = start[warp].x, len = start[warp].z, tiles = (len - 1) / kTile + 1;
+    int sub = start[warp].y / tiles, tile = start[warp].y - sub * tiles, left = todo;
+    int head = sub / lay.chunks, chunk = sub - head * lay.chunks;
+    const int* table = c.table + (long long)start[warp].w * c.width;
     int block = __ldg(table + tile / (kBlock / kTile));
 
-    const int lane_token = lane / 8, lane_chunk = lane % 8;  // a copy: 4 tokens x 8 chunks of 16 bytes
+    // a copy: 4 tokens x 8 chunks of 16 bytes; chunk x of token t lies at x ^ (t % 8), so that fragments are read
+    // without bank conflicts
+    const int lane_token = lane / 8;
+    const unsigned to_even = smem_u32(ring) + lane_token * kHead + (((lane % 8) ^ lane_token) << 4);
+    const unsigned to_odd = to_even ^ 64;
     auto load = [&](int stage) {
       if (left > 0) {
-        const bool bad = block < 0 || block >= c.n_blocks;
-        const long long at = (long long)(bad ? 0 : block) * c.heads + lay.head(sub);
+        const bool bad = (unsigned)block >= (unsigned)c.n_blocks;
+        const long long at = (long long)(bad ? 0 : block) * c.heads + head;
         const int valid = min(kTile, len - tile * kTile);
         if (lane == 0) {
-          notes[stage] = {(long long)row * lay.subs + sub, valid,
-                          (tile == 0 ? kFirst : 0) | (tile == tiles - 1 ? kLast : 0) | (bad ? kBad : 0)};
+          notes[stage] = {row, sub, valid, (tile == 0 ? kFirst : 0) | (tile == tiles - 1 ? kLast : 0) | (bad ? kBad : 0)};
           if (bad) bad_index();
         }
-        if (lane < 2) copy4(smem_u32(scales + stage * 2 + lane), c.scales[lane] + at);
-        const long long from = (at * kBlock + tile % (kBlock / kTile) * kTile) * kHead + lane * 16;
+        if (lane < 2) copy4(smem_u32(scales + stage * 2 + lane), (lane ? c.scales[1] : c.scales[0]) + at);
+        const long long from = at * (kBlock * kHead) + tile % (kBlock / kTile) * kTileBytes + lane * 16;
         const int8_t* k = c.codes[0] + from;
         const int8_t* v = c.codes[1] + from;
-        const unsigned to = smem_u32(ring + stage * kStageBytes) + lane_token * kHead;
+        const unsigned off = stage * kStageBytes;
+        if (valid == kTile) {
 #pragma unroll
-        for (int i = 0; i < kTile / 4; ++i) {
-          // chunk x of token t lies at x ^ (t % 8): no bank conflicts when fragments are read
-          const unsigned off = to + i * 4 * kHead + ((lane_chunk ^ (i % 2 * 4 + lane_token)) << 4);
-          if (i * 4 + lane_token < valid) {
-            copy16(off, k + i * 4 * kHead);
-            copy16(off + kTileBytes, v + i * 4 * kHead);
+          for (int i = 0; i < kTile / 4; ++i) {
+            const unsigned to = (i % 2 ? to_odd : to_even) + off + i * 4 * kHead;
+            copy16(to, k + i * 4 * kHead);
+            copy16(to + kTileBytes, v + i * 4 * kHead);
+          }
+        } else {
+          for (int i = 0; i < kTile / 4; ++i) {
+            const unsigned to = (i % 2 ? to_odd : to_even) + off + i * 4 * kHead;
+            if (i * 4 + lane_token < valid) {
+              copy16(to, k + i * 4 * kHead);
+              copy16(to + kTileBytes, v + i * 4 * kHead);
+            }
           }
         }
         // the next tile, its block's id one step ahead of its use
         if (--left > 0) {
           if (++tile == tiles) {
             tile = 0;
-            if (++sub == lay.subs) {
-              sub = 0;
-              do {
-                ++row;
-                tiles = row_tiles(c, a, row);
-              } while (tiles == 0);
-              len = __ldg(a.row_len + row);
-              table = c.table + (long long)__ldg(a.row_seq + row) * c.width;
+            ++sub;
+            if (++chunk == lay.chunks) {
+              chunk = 0;
+              if (++head == c.heads) {
+                head = sub = 0;
+                do {
+                  ++row;
+                  tiles = row_tiles(c, a, row);
+                } while (tiles == 0);
+                len = __ldg(a.row_len + row);
+                table = c.table + (long long)__ldg(a.row_seq + row) * c.width;
+              }
             }
           }
           block = __ldg(table + tile / (kBlock / kTile));
@@ -242,48 +293,50 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
       }
       copies_commit();
     };
+
+    Query q;
+    auto load_query = [&](int it_row, int it_sub) {
+      float4 x[8];
+      float top = 0.0f;
+      const T* from = static_cast<const T*>(a.q) + it_row * a.q_stride + (long long)(lay.first_q(it_sub) + g) * kHead + q4 * 32;
+      const bool live = g < lay.count(it_sub);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        x[s] = live ? load4(from + s * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[s].x), fabsf(x[s].y)), fmaxf(fabsf(x[s].z), fabsf(x[s].w))));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e and 2^e with the row's largest value in [1, 2) after the scaling
+      const int e = top == 0.0f ? 127 : min(253, max(1, (int)(__float_as_uint(top) >> 23)));
+      const float down = __uint_as_float((unsigned)(254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
+      q.scale = a.scale * up * 1.4426950408889634f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        split_half(x[s].x * down, x[s].y * down, q.f[s][0], q.f[s][1]);
+        split_half(x[s].z * down, x[s].w * down, q.f[s][2], q.f[s][3]);
+      }
+    };
+
+    int it_row = row, it_sub = sub;
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) load(s);
+    load_query(it_row, it_sub);  // while the first tiles are on their way
 
-    unsigned qf[8][4];          // q in fragments: dims 32 q4 + 4 s + {0, 1 | 2, 3} of head g, high and low
-    float qs = 0.0f;            // scale * log2(e) * the power of two that was taken out of q
-    float m = 0.0f, l = 0.0f;   // head g: maximum (base 2) and this lane's share of the sum
-    float o[16][2];             // head g: dims 32 q4 + j and 32 q4 + 16 + j
-    bool whole = false;
-    long long item = -1;
+    float m = -INFINITY, l = 0.0f;  // head g: maximum (base 2) and this lane's share of the sum
+    unsigned long long o[16];       // head g: dims 32 q4 + j and 32 q4 + 16 + j
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = 0;
+    bool fresh = true, whole = false;
     int stage = 0;
-    for (long long t = 0; t < todo; ++t) {
+    for (int t = 0; t < todo; ++t) {
       copies_wait<kStages - 2>();
       __syncwarp();
       const Note note = notes[stage];
-      if (note.item != item) {
-        item = note.item;
+      if (fresh) {
+        fresh = false;
         whole = note.flags & kFirst;
-        const int it_row = (int)(item / lay.subs), it_sub = (int)(item % lay.subs);
-        float4 q[8];
-        float top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          q[s] = g < lay.count(it_sub) ? load4(static_cast<const T*>(a.q) + it_row * a.q_stride +
-                                               (long long)(lay.first_q(it_sub) + g) * kHead + q4 * 32 + s * 4)
-                                       : make_float4(0.f, 0.f, 0.f, 0.f);
-          top = fmaxf(top, fmaxf(fmaxf(fabsf(q[s].x), fabsf(q[s].y)), fmaxf(fabsf(q[s].z), fabsf(q[s].w))));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^-e and 2^e with the row's largest value in [1, 2) after the scaling
-        const int e = top == 0.0f ? 127 : min(253, max(1, (int)(__float_as_uint(top) >> 23)));
-        const float down = __uint_as_float((unsigned)(254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
-        qs = a.scale * up * 1.4426950408889634f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          split_half(q[s].x * down, q[s].y * down, qf[s][0], qf[s][1]);
-          split_half(q[s].z * down, q[s].w * down, qf[s][2], qf[s][3]);
-        }
-        m = -INFINITY;
-        l = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = 0.0f;
+        if (note.row != it_row || note.sub != it_sub) load_query(it_row = note.row, it_sub = note.sub);
       }
       const uint8_t* kt = ring + stage * kStageBytes;
       const uint8_t* vt = kt + kTileBytes;
@@ -293,40 +346,49 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
       // codes of token 8 j + g are two 16-byte chunks, four codes for each of the 8 steps
       float s[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-        const uint8_t* kr = kt + (j * 8 + g) * kHead;
+      for (int h = 0; h < 2; ++h) {
+        uint4 b[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 b = *reinterpret_cast<const uint4*>(kr + (((q4 * 2 + h) ^ g) << 4));
-          const unsigned w[4] = {b.x ^ 0x80808080u, b.y ^ 0x80808080u, b.z ^ 0x80808080u, b.w ^ 0x80808080u};
+        for (int j = 0; j < 4; ++j)
+          b[j] = *reinterpret_cast<const uint4*>(kt + (j * 8 + g) * kHead + (((q4 * 2 + h) ^ g) << 4));
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mma(s[j], qf[h * 4 + i], codes_to_half2<0x5150>(w[i]), codes_to_half2<0x5352>(w[i]));
-        }
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const unsigned w = reinterpret_cast<const unsigned*>(&b[j])[i] ^ 0x80808080u;
+            const unsigned b0 = codes_to_half2<0x5150>(w), b1 = codes_to_half2<0x5352>(w);
+            if (h == 0 && i == 0) mma_first(s[j], q.f[0], b0, b1);
+            else mma(s[j], q.f[h * 4 + i], b0, b1);
+          }
       }
-      const float cs = qs * ks;
+      const float cs = q.scale * ks;
       float p[4][2], tm = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          p[j][i] = j * 8 + q4 * 2 + i < note.valid ? (s[j][i] + s[j][i + 2]) * cs : -INFINITY;
-          tm = fmaxf(tm, p[j][i]);
-        }
+        for (int i = 0; i < 2; ++i) p[j][i] = (s[j][i] + s[j][i + 2]) * cs;
+      if (note.valid < kTile) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (j * 8 + q4 * 2 + i >= note.valid) p[j][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tm = fmaxf(tm, fmaxf(p[j][0], p[j][1]));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
       float tl = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          p[j][i] = ex2(p[j][i] - tm);
-          tl += p[j][i];
-        }
+        for (int i = 0; i < 2; ++i) p[j][i] = ex2(p[j][i] - tm);
+        tl += p[j][0] + p[j][1];
+      }
       const float mn = fmaxf(m, tm), keep = ex2(m - mn), add = ex2(tm - mn), av = add * vs;
       m = mn;
       l = l * keep + add * tl;
+      const unsigned long long keep2 = pair(keep, keep), av2 = pair(av, av);
 
       // weights of two 8-token columns are the operand of one 16-token step
       unsigned pf[2][4];
@@ -347,8 +409,6 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
       for (int w = 0; w < 4; ++w) {
         float d[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.0f;
-#pragma unroll
         for (int k = 0; k < 2; ++k) {
           unsigned b[2][4];
 #pragma unroll
@@ -362,34 +422,34 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
             b[i][3] = codes_to_half2<0x5352>(hi);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma(d[i], pf[k], b[0][i], b[1][i]);
+          for (int i = 0; i < 4; ++i) {
+            if (k == 0) mma_first(d[i], pf[0], b[0][i], b[1][i]);
+            else mma(d[i], pf[1], b[0][i], b[1][i]);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[w * 4 + i][0] = fmaf(av, d[i][0] + d[i][2], o[w * 4 + i][0] * keep);
-          o[w * 4 + i][1] = fmaf(av, d[i][1] + d[i][3], o[w * 4 + i][1] * keep);
-        }
+        for (int i = 0; i < 4; ++i)
+          o[w * 4 + i] = fma2(av2, add2(pair(d[i][0], d[i][1]), pair(d[i][2], d[i][3])), mul2(o[w * 4 + i], keep2));
       }
 
       __syncwarp();  // the stage that is refilled next was read one step ago
-      load((stage + kStages - 1) % kStages);
+      load(stage == 0 ? kStages - 1 : stage - 1);
       stage = stage + 1 == kStages ? 0 : stage + 1;
 
       const bool ends = note.flags & kLast;
       if (ends || t == todo - 1) {
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const int it_sub = (int)(item % lay.subs);
         if (whole && ends) {
           if (g < lay.count(it_sub)) {
-            const long long it_row = item / lay.subs;
             const int h = lay.first_q(it_sub) + g;
             const float r = 1.0f / l;
 #pragma unroll
-            for (int j = 0; j < 16; j += 4)
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                put_out<T>(a, it_row, h, q4 * 32 + i * 16 + j, make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]), r);
+            for (int j = 0; j < 16; j += 4) {
+              const float2 x[4] = {unpair(o[j]), unpair(o[j + 1]), unpair(o[j + 2]), unpair(o[j + 3])};
+              put_out<T>(a, it_row, h, q4 * 32 + j, make_float4(x[0].x, x[1].x, x[2].x, x[3].x), r);
+              put_out<T>(a, it_row, h, q4 * 32 + 16 + j, make_float4(x[0].y, x[1].y, x[2].y, x[3].y), r);
+            }
             if (q4 == 0) put_lse(a, it_row, h, m, l);
           }
         } else {
@@ -400,77 +460,86 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
           }
           float* to = whole ? reinterpret_cast<float*>(ring) : part;
 #pragma unroll
-          for (int j = 0; j < 16; j += 4)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              *reinterpret_cast<float4*>(to + g * kHead + q4 * 32 + i * 16 + j) =
-                  make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
+          for (int j = 0; j < 16; j += 4) {
+            const float2 x[4] = {unpair(o[j]), unpair(o[j + 1]), unpair(o[j + 2]), unpair(o[j + 3])};
+            *reinterpret_cast<float4*>(to + g * kHead + q4 * 32 + j) = make_float4(x[0].x, x[1].x, x[2].x, x[3].x);
+            *reinterpret_cast<float4*>(to + g * kHead + q4 * 32 + 16 + j) = make_float4(x[0].y, x[1].y, x[2].y, x[3].y);
+          }
           if (q4 == 0) {
             to[kRows * kHead + g] = m;
             to[kRows * kHead + kRows + g] = l;
           }
           if (lane == 0) {
-            part_item[warp][whole] = item;
+            part_item[2 * warp + whole] = it_row * lay.subs + it_sub;
             if (!whole) part_ended[warp] = ends;
           }
         }
-        item = -1;
+        fresh = true;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = 0;
       }
     }
     copies_wait<0>();
   }
   __syncthreads();
 
-  // ---- join the warps' parts: part 2 w is warp w's item from before, part 2 w + 1 the one that goes on
-  if (threadIdx.x < 2) info[2 * blockIdx.x + threadIdx.x] = -1;
-  __syncthreads();
-  auto part_at = [&](int p) {
-    return p % 2 ? reinterpret_cast<const float*>(smem + p / 2 * kStages * kStageBytes)
-                 : reinterpret_cast<const float*>(smem + kPartsOffset) + p / 2 * kPartFloats;
-  };
-  for (int first = 2 * warp; first < 2 * warp + 2; ++first) {
-    const long long item = part_item[warp][first % 2];
-    if (item < 0) continue;
-    int prev = first - 1;
-    while (prev >= 0 && part_item[prev / 2][prev % 2] < 0) --prev;
-    if (prev >= 0 && part_item[prev / 2][prev % 2] == item) continue;  // joined by an earlier part's warp
-    bool ended = first % 2 == 0 && part_ended[warp];
-    int last = first;
-    for (int p = first + 1; p < 2 * kWarps && !ended; ++p) {
-      if (part_item[p / 2][p % 2] < 0) continue;
-      if (part_item[p / 2][p % 2] != item) break;
-      last = p;
-      ended = p % 2 == 0 && part_ended[p / 2];
+  // ---- join the warps' parts, warp h head h: part 2 w is warp w's item from before, part 2 w + 1 the one that goes on
+  int* info = reinterpret_cast<int*>(static_cast<uint8_t*>(a.work) + kInfoOffset) + 2 * blockIdx.x;
+  const int my_item = lane < 2 * kWarps ? part_item[lane] : -1;
+  const float* my_part = lane % 2 ? reinterpret_cast<const float*>(smem + lane / 2 % kWarps * kStages * kStageBytes)
+                                  : reinterpret_cast<const float*>(smem + kPartsOffset) + lane / 2 % kWarps * kPartFloats;
+  const unsigned live = __ballot_sync(0xffffffffu, my_item >= 0);
+  const unsigned earlier = live & ((1u << lane) - 1);
+  const int prev_item = __shfl_sync(0xffffffffu, my_item, earlier ? 31 - __clz(earlier) : 0);
+  unsigned firsts = __ballot_sync(0xffffffffu, my_item >= 0 && !(earlier && prev_item == my_item));
+  int before_info = -1, after_info = -1;
+  while (firsts) {
+    const int first = __ffs(firsts) - 1;
+    firsts &= firsts - 1;
+    const unsigned members = live & (firsts ? (firsts & -firsts) - 1 : ~0u) & ~((1u << first) - 1);
+    const int last = 31 - __clz(members), item = __shfl_sync(0xffffffffu, my_item, first);
+    const bool ended = last % 2 == 0 && part_ended[last / 2], done = first % 2 == 1 && ended;
+    if (!done) {
+      if (first % 2) after_info = item;
+      else before_info = 2 * item + ended;
     }
-    const int it_sub = (int)(item % lay.subs);
-    const bool done = first % 2 == 1 && ended;
-    const int slot = 2 * blockIdx.x + first % 2;
-    for (int h = 0; h < lay.count(it_sub); ++h) {
-      float m = -INFINITY, l = 0.0f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int p = first; p <= last; ++p)
-        if (part_item[p / 2][p % 2] == item) m = fmaxf(m, part_at(p)[kRows * kHead + h]);
-      for (int p = first; p <= last; ++p) {
-        if (part_item[p / 2][p % 2] != item) continue;
-        const float* x = part_at(p);
-        const float f = ex2(x[kRows * kHead + h] - m);
-        const float4 v = *reinterpret_cast<const float4*>(x + h * kHead + lane * 4);
-        l = fmaf(f, x[kRows * kHead + kRows + h], l);
-        o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
-      }
-      if (done) {
-        put_out<T>(a, item / lay.subs, lay.first_q(it_sub) + h, lane * 4, o, 1.0f / l);
-        if (lane == 0) put_lse(a, item / lay.subs, lay.first_q(it_sub) + h, m, l);
-      } else {
-        float* to = work + (size_t)slot * kPartFloats;
-        *reinterpret_cast<float4*>(to + h * kHead + lane * 4) = o;
-        if (lane == 0) {
-          to[kRows * kHead + h] = m;
-          to[kRows * kHead + kRows + h] = l;
-        }
+    const int it_row = item / lay.subs, it_sub = item - it_row * lay.subs;
+    if (warp >= lay.count(it_sub)) continue;
+    const bool member = members >> lane & 1;
+    const float pm = member ? my_part[kRows * kHead + warp] : -INFINITY;
+    float m = pm;
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+    const float f = member ? ex2(pm - m) : 0.0f;
+    float l = member ? f * my_part[kRows * kHead + kRows + warp] : 0.0f;
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (unsigned rest = members; rest; rest &= rest - 1) {
+      const int p = __ffs(rest) - 1;
+      const float* x = p % 2 ? reinterpret_cast<const float*>(smem + p / 2 * kStages * kStageBytes)
+                             : reinterpret_cast<const float*>(smem + kPartsOffset) + p / 2 * kPartFloats;
+      const float4 v = *reinterpret_cast<const float4*>(x + warp * kHead + lane * 4);
+      const float fp = __shfl_sync(0xffffffffu, f, p);
+      o = make_float4(fmaf(fp, v.x, o.x), fmaf(fp, v.y, o.y), fmaf(fp, v.z, o.z), fmaf(fp, v.w, o.w));
+    }
+    if (done) {
+      put_out<T>(a, it_row, lay.first_q(it_sub) + warp, lane * 4, o, 1.0f / l);
+      if (lane == 0) put_lse(a, it_row, lay.first_q(it_sub) + warp, m, l);
+    } else {
+      float* to = static_cast<float*>(a.work) + (size_t)(2 * blockIdx.x + first % 2) * kPartFloats;
+      *reinterpret_cast<float4*>(to + warp * kHead + lane * 4) = o;
+      if (lane == 0) {
+        to[kRows * kHead + warp] = m;
+        to[kRows * kHead + kRows + warp] = l;
       }
     }
-    if (!done && lane == 0) info[slot] = first % 2 ? item : 2 * item + ended;
+  }
+  if (threadIdx.x == 0) {
+    info[0] = before_info;
+    info[1] = after_info;
   }
 
   // ---- rows without a tile: nothing cached yet, or an index that is no row of the cache
@@ -488,62 +557,61 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
 }
 
 // Joins the parts of an item that several CTAs' runs share: block (c, h) takes the item that began in CTA c and went
-// on, head h of it. Four warps take every fourth part each, so that their loads overlap.
+// on, head h of it. A warp takes every eighth part, its loads independent of one another.
 template <int kType>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(Cache c, Attend a) {
   using T = typename TypeOf<kType>::T;
-  __shared__ float4 sum[kMergeThreads / 32][32];
-  __shared__ float weight[kMergeThreads / 32], top[kMergeThreads / 32];
+  constexpr int kMergeWarps = kMergeThreads / 32;
+  __shared__ float4 sum[kMergeWarps][32];
+  __shared__ float top[kMergeWarps], total[kMergeWarps], factor[kCtas];
+  static_assert(kCtas <= kMergeThreads, "a thread per part");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Layout lay(c, a);
   const float* work = static_cast<const float*>(a.work);
-  const long long* info = reinterpret_cast<const long long*>(static_cast<const uint8_t*>(a.work) + kInfoOffset);
+  const int* info = reinterpret_cast<const int*>(static_cast<const uint8_t*>(a.work) + kInfoOffset);
   const int cta = blockIdx.x, h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const long long item = info[2 * cta + 1];
-  if (item < 0 || h >= lay.count((int)(item % lay.subs))) return;
-  // parts: 2 cta + 1, then the first ones of the CTAs behind up to the one where the item ends
-  int n = 1;
-  for (int base = cta + 1; base < kCtas; base += 32) {
-    const long long x = base + lane < kCtas ? info[2 * (base + lane)] : -1;
-    const unsigned end = __ballot_sync(0xffffffffu, x != 2 * item);  // ends there, or is another's
-    n += end ? __ffs(end) - 1 : 32;
-    if (end) {
-      if (__shfl_sync(0xffffffffu, x, __ffs(end) - 1) == 2 * item + 1) ++n;
-      break;
-    }
-  }
-  auto part = [&](int i) { return work + (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kPartFloats; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kMergeThreads) m = fmaxf(m, part(i)[kRows * kHead + h]);
+  const int item = info[2 * cta + 1];
+  if (item < 0) return;
+  const Layout lay(c, a);
+  const int it_row = item / lay.subs, it_sub = item - it_row * lay.subs;
+  if (h >= lay.count(it_sub)) return;
+  // part 0 is 2 cta + 1, part i the first one of CTA cta + i, up to the CTA where the item ends
+  const int i = threadIdx.x, x = i > 0 && cta + i < kCtas ? info[2 * (cta + i)] : -1;
+  const bool mine = i == 0 || x >> 1 == item;
+  const float* my_part = work + (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kPartFloats;
+  const float pm = mine ? my_part[kRows * kHead + h] : -INFINITY, pl = mine ? my_part[kRows * kHead + kRows + h] : 0.0f;
+  float m = pm;
 #pragma unroll
-  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
   if (lane == 0) top[warp] = m;
-  __syncthreads();
+  const int n = __syncthreads_count(mine);
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 32; ++w) m = fmaxf(m, top[w]);
-  float l = 0.0f;
+  for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, top[w]);
+  const float f = mine ? ex2(pm - m) : 0.0f;
+  if (i < kCtas) factor[i] = f;
+  float l = mine ? f * pl : 0.0f;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+  if (lane == 0) total[warp] = l;
+  __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = warp; i < n; i += kMergeThreads / 32) {
-    const float* x = part(i);
-    const float f = ex2(x[kRows * kHead + h] - m);
-    const float4 v = *reinterpret_cast<const float4*>(x + h * kHead + lane * 4);
-    l = fmaf(f, x[kRows * kHead + kRows + h], l);
-    o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
+#pragma unroll 10
+  for (int p = warp; p < n; p += kMergeWarps) {
+    const float4 v = *reinterpret_cast<const float4*>(work + (size_t)(2 * (cta + p) + (p == 0)) * kPartFloats + h * kHead + lane * 4);
+    const float fp = factor[p];
+    o = make_float4(fmaf(fp, v.x, o.x), fmaf(fp, v.y, o.y), fmaf(fp, v.z, o.z), fmaf(fp, v.w, o.w));
   }
   sum[warp][lane] = o;
-  if (lane == 0) weight[warp] = l;
   __syncthreads();
   if (warp != 0) return;
+  l = total[0];
 #pragma unroll
-  for (int w = 1; w < kMergeThreads / 32; ++w) {
+  for (int w = 1; w < kMergeWarps; ++w) {
     const float4 v = sum[w][lane];
-    l += weight[w];
+    l += total[w];
     o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
   }
-  const int q_head = lay.first_q((int)(item % lay.subs)) + h;
-  put_out<T>(a, item / lay.subs, q_head, lane * 4, o, 1.0f / l);
-  if (lane == 0) put_lse(a, item / lay.subs, q_head, m, l);
+  put_out<T>(a, it_row, lay.first_q(it_sub) + h, lane * 4, o, 1.0f / l);
+  if (lane == 0) put_lse(a, it_row, lay.first_q(it_sub) + h, m, l);
 }
 
 template <int kType>
