@@ -8,13 +8,14 @@
 // w = exp(-b/64) (1 - q 2^-23) with the integer q = rint(2^23 (1 - exp(-f))), f = z - b/64. One pass adds up the
 // count and the q of every bucket, as integers, so neither the sums nor the token depend on the order of the
 // atomics. The bucket sums (in 64 bits) tell in which bucket each filter's border and the drawn number fall, and only
-// tokens of such buckets are gathered and sorted. A weight is off by at most 2^-24 of its bucket's largest (the
-// rounding of q; f is exact to 2^-30).
+// tokens of such buckets are gathered and sorted. A weight is off by at most 2^-24 of its bucket's largest, and at
+// random: f is exact to 2^-30, which a drawn number that falls between 150000 small weights needs.
 //
-// One cluster of 8 CTAs takes a row, an eighth of the logits each, in shared memory: they are read from HBM once. Small
-// vocabularies take one CTA. The first CTA leads: it reads the others' bucket sums through distributed shared
-// memory, decides, and asks for what it needs to see. Bound: the latency of those steps for few rows (8 SMs of 148
-// work on a row), bytes for many.
+// A row is read three times: for its maximum, for the bucket sums, for the tokens to sort; the second and third
+// reading mostly meet L2. A cluster of 8 CTAs shares a row, fewer when there are rows enough to fill the GPU with
+// two CTAs per SM. The first CTA leads: it reads the others' bucket sums through distributed shared memory, decides
+// (every thread the same way, by bisection, without barriers) and asks for what it needs to see. Bound: for few rows
+// the latency of those steps, for many the ~35 instructions and two shared atomics per logit of the second pass.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,9 +37,11 @@ constexpr int kBuckets = 2048;
 constexpr int kPerThread = kBuckets / kThreads;
 constexpr int kList = 1024;  // tokens that are sorted at once
 constexpr int kOrderBits = 50;
-constexpr int kDigit = 11;   // bits by which a crowded bucket is narrowed at a time
-constexpr int kCluster = 8;
-constexpr int kOneCta = 8192;  // vocabularies up to this size take one CTA: less to read than a cluster costs to sync
+constexpr int kDigit = 11;        // bits by which a crowded bucket is narrowed at a time
+constexpr int kFold = 1 << 15;    // logits whose q, below 2^17 each, fit a 32-bit sum
+constexpr int kMaxCluster = 8;
+constexpr int kOneCta = 8192;     // vocabularies up to this size take one CTA: less to read than a cluster costs to sync
+constexpr int kResident = 2 * 148;  // CTAs that fit the GPU at once
 
 typedef unsigned long long u64;
 
@@ -71,38 +74,40 @@ __device__ __forceinline__ u64 order_of(float x, int i) { return (u64)key_of(x) 
 __device__ __forceinline__ int index_of(u64 order) { return kMaxVocab - 1 - (int)(order & (kMaxVocab - 1)); }
 __device__ __forceinline__ float value_of(u64 order) { return value_of((unsigned)(order >> 18)); }
 
-// z = (top - x) / temperature in parts: bucket and q. The product with 1 / temperature = c + c_low is exact to
+// 64 z = 64 (top - x) / temperature in parts: bucket and q. The product with 64 / temperature = c + c_low is exact to
 // about 2^-48, and so is its distance to the bucket's border.
 struct Scale {
   float top, c, c_low;
-  __device__ Scale(float top_, float t) : top(top_), c(1.0f / t) {
-    c_low = c > 0.0f ? fmaf(-t, c, 1.0f) * c : 0.0f;
-    if (!(fabsf(c_low) < c)) c_low = 0.0f;
+  __device__ Scale() {}
+  __device__ Scale(float top_, float t) : top(top_) {
+    const float r = 1.0f / t;
+    float low = r > 0.0f ? fmaf(-t, r, 1.0f) * r : 0.0f;
+    if (!(fabsf(low) < r)) low = 0.0f;
+    c = fminf(64.0f * r, 3.4028235e38f);  // finite, so that the best token stays at 0 steps
+    c_low = 64.0f * low;
   }
+  __device__ __forceinline__ float steps(float x) const { return (top - x) * c; }
+  static __device__ __forceinline__ bool counts(float steps) { return steps < (float)kBuckets; }  // false for NaN
   // the bucket, or -1 for a weight that counts as 0
-  __device__ __forceinline__ int bucket(float x, float& d) const {
-    d = x == top ? 0.0f : top - x;  // +infinity ties with itself
-    const float t = d * c * 64.0f;
-    return t < (float)kBuckets ? (int)t : -1;
-  }
   __device__ __forceinline__ int bucket(float x) const {
-    float d;
-    return bucket(x, d);
+    const float t = steps(x);
+    return counts(t) ? (int)t : -1;
   }
-  __device__ __forceinline__ int part(float x, float d, int b) const {
-    const float s = d == 0.0f ? 0.0f : top - d;  // what x is short of top - d, exactly (two-sum)
-    const float low = d == 0.0f ? 0.0f : (top - (s + d)) - (x - s);
-    float f = fmaf(d, c, -(float)b * (1.0f / 64.0f)) + fmaf(d, c_low, low * c);
-    f = fmaxf(f, 0.0f);
-    // 1 - exp(-f) for f < 1/64: the series' next term, f^5 / 120, is below 2^-36
-    const float e = f * fmaf(f, fmaf(f, fmaf(f, -1.0f / 24.0f, 1.0f / 6.0f), -0.5f), 1.0f);
-    return min(__float2int_rn(e * 8388608.0f), 131071);
+  // q + kQBits, for a logit in bucket b (both conversions by adding 1.5 * 2^23, not on the slow pipe)
+  static constexpr unsigned kQBits = 0x4b400000u;
+  __device__ __forceinline__ unsigned part_bits(float x, float b) const {
+    const float d = top - x, s = top - d;
+    const float low = (top - (s + d)) - (x - s);  // d + low is top - x exactly (two-sum)
+    float f = fmaf(d, c, -b) + fmaf(d, c_low, low * c);
+    f = fminf(fmaxf(f, 0.0f), 1.0f);
+    // 2^23 (1 - exp(-f / 64)); the series' next term is below 2^-36
+    constexpr float k1 = 131072.0f, k2 = -1024.0f, k3 = 16.0f / 3.0f, k4 = -1.0f / 48.0f;
+    return __float_as_uint(fmaf(f, fmaf(f, fmaf(f, fmaf(f, k4, k3), k2), k1), 12582912.0f));
   }
   // the weight in 64 bits, as the sums have it
   __device__ double weight(float x) const {
-    float d;
-    const int b = bucket(x, d);
-    return b < 0 ? 0.0 : exp(-(double)b / 64.0) * (double)(8388608 - part(x, d, b)) * (1.0 / 8388608.0);
+    const int b = bucket(x);
+    return b < 0 ? 0.0 : exp(-(double)b / 64.0) * (double)(8388608u - (part_bits(x, (float)b) - kQBits)) * (1.0 / 8388608.0);
   }
 };
 
@@ -114,46 +119,74 @@ struct Command {
   u64 prefix;           // their value
 };
 
+struct Sums {
+  unsigned count[kBuckets];
+  u64 q[kBuckets];
+};
+// Running sums up to and with each bucket.
+struct Running {
+  unsigned count[kBuckets];
+  double mass[kBuckets];
+  // the first bucket at which the count or the mass suffices (one with tokens in it), the last one if none does
+  __device__ int find_count(unsigned k) const {
+    int lo = 0, hi = kBuckets - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (count[mid] >= k) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
+  }
+  __device__ int find_mass(double want, bool more) const {
+    int lo = 0, hi = kBuckets;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (more ? mass[mid] > want : mass[mid] >= want) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo < kBuckets ? lo : find_count(count[kBuckets - 1]);
+  }
+  __device__ unsigned before(int b) const { return b ? count[b - 1] : 0; }
+  __device__ double mass_before(int b) const { return b ? mass[b - 1] : 0.0; }
+};
+
 struct Shared {
-  u64 best[kCluster];
+  union {
+    unsigned hist[2][kBuckets];  // counts, sums of q + kQBits modulo 2^32
+    struct {
+      u64 list[kList];
+      double prefix[kList];
+    };
+  };
+  Sums sums;       // this CTA's
+  Running row;     // the leader's: of all CTAs
+  Running bins;    // the leader's: of the bins of a crowded bucket, best first
+  u64 best[kMaxCluster];
   Command command;
   int listed, counted;
   u64 warp_best[kWarps];
   double warp_mass[kWarps];
   unsigned warp_count[kWarps];
-  int found;
-  double answer_mass;
-  unsigned answer_count;
-  double bucket_mass;
-  unsigned bucket_count;
 };
 
-// A border or a draw inside one bucket, or the whole kept set: how many tokens up to and with the found one.
+// What is kept so far: everything before a bucket, and the first tokens of the bucket itself.
 struct Cut {
   int bucket;
-  unsigned count;  // tokens of the bucket that are kept
-  double mass;     // of everything up to there
+  unsigned count;
+  double mass;  // of all that
 };
 
 template <int kType, int kCl>
 struct Row {
   using T = typename TypeOf<kType>::T;
-  const Sample& a;
   Shared& sh;
-  float* x;             // this CTA's logits; NaN as -infinity
-  unsigned* hist;       // [2][kBuckets]: counts, sums of q
-  u64* list;            // [kList], in the histogram's place
-  double* prefix;       // [kList], behind it
-  int rank, lo, n;
-  Scale scale{0.0f, 1.0f};
-  double least = 0.0, temperature = 1.0;
-  // the leader's bucket sums, kPerThread buckets a thread
-  unsigned count[kPerThread], count_before;
-  double mass[kPerThread], mass_before;
-  unsigned all_count;
-  double all_mass;
+  const T* x;  // this CTA's logits
+  int lo, n;   // the first one's index, their number
+  Scale scale;
+  bool top_infinite;
+  float least, temperature;
 
-  __device__ Row(const Sample& a_, Shared& s_) : a(a_), sh(s_) {}
+  __device__ explicit Row(Shared& s) : sh(s) {}
 
   __device__ __forceinline__ void sync_all() {
     if (kCl > 1) cg::this_cluster().sync();
@@ -165,61 +198,108 @@ struct Row {
     return p;
   }
 
-  // ---- work of every CTA
-  __device__ void add_up(const Command& cmd) {
-    const int shift = kOrderBits - cmd.bits, digit = min(kDigit, shift);
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float v = x[i];
-      if (!(v > -INFINITY)) continue;
-      float d;
-      const int b = scale.bucket(v, d);
-      if (b < cmd.first || b > cmd.last) continue;
-      const u64 o = order_of(v, lo + i);
-      if (cmd.bits && o >> shift != cmd.prefix) continue;
-      const int bin = cmd.first == cmd.last ? (int)(o >> (shift - digit)) & ((1 << digit) - 1) : b;
-      atomicAdd(hist + bin, 1u);
-      atomicAdd(hist + kBuckets + bin, (unsigned)scale.part(v, d, b));
+  // f(logit, its place in x) for places from .. to - 1 of this CTA's logits: 16-byte loads, four at a time, between the
+  // first and the last aligned place.
+  template <typename F>
+  __device__ __forceinline__ void for_each(int from, int to, F f) {
+    constexpr int kVec = 16 / (int)sizeof(T), kAhead = 4;
+    const int head = min(to - from, (int)((16 - reinterpret_cast<uintptr_t>(x + from) % 16) % 16 / sizeof(T)));
+    const int vecs = (to - from - head) / kVec, tail = from + head + vecs * kVec;
+    if ((int)threadIdx.x < head) f(to_float(x[from + threadIdx.x]), from + (int)threadIdx.x);
+    if ((int)threadIdx.x < to - tail) f(to_float(x[tail + threadIdx.x]), tail + (int)threadIdx.x);
+    const uint4* v = reinterpret_cast<const uint4*>(x + from + head);
+    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kAhead) {
+      uint4 b[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (i0 + k * kThreads < vecs) b[k] = __ldg(v + i0 + k * kThreads);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (i0 + k * kThreads >= vecs) break;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          f(to_float(reinterpret_cast<const T*>(&b[k])[e]), from + head + (i0 + k * kThreads) * kVec + e);
+      }
     }
   }
+  // a logit as the sums see it: where the largest is +infinity, one of 0 and nothing beside it
+  __device__ __forceinline__ float seen(float v) const { return top_infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v; }
+
+  // ---- work of every CTA
   __device__ void clear_histogram() {
-    for (int i = threadIdx.x; i < 2 * kBuckets; i += kThreads) hist[i] = 0;
+    for (int i = threadIdx.x; i < 2 * kBuckets; i += kThreads) sh.hist[0][i] = 0;
     __syncthreads();
+  }
+  // Counts and q of every bucket, or of the bins of one bucket, into sh.sums.
+  template <bool kBins>
+  __device__ void add_up(const Command& cmd) {
+    unsigned c[kPerThread] = {};
+    u64 q[kPerThread] = {};
+    const int shift = kOrderBits - cmd.bits, digit = min(kDigit, shift);
+    const int first = threadIdx.x * kPerThread;
+    for (int from = 0; from < max(n, 1); from += kFold) {
+      clear_histogram();
+      for_each(from, min(n, from + kFold), [&](float v, int i) {
+        v = seen(v);
+        const float t = scale.steps(v);
+        if (!Scale::counts(t)) return;
+        const float up = __fadd_rd(t, 8388608.0f);  // floor(t) in the low bits
+        const int b = __float_as_uint(up) & (2 * kBuckets - 1);
+        int bin = b;
+        if (kBins) {
+          const u64 o = order_of(v + 0.0f, lo + i);
+          if (b != cmd.first || (cmd.bits && o >> shift != cmd.prefix)) return;
+          bin = (int)(o >> (shift - digit)) & ((1 << digit) - 1);
+        }
+        atomicAdd(&sh.hist[0][bin], 1u);
+        atomicAdd(&sh.hist[1][bin], scale.part_bits(v, up - 8388608.0f));
+      });
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) {
+        const unsigned k = sh.hist[0][first + i];
+        c[i] += k;
+        q[i] += sh.hist[1][first + i] - k * Scale::kQBits;  // modulo 2^32, which the sum of q is below
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      sh.sums.count[first + i] = c[i];
+      sh.sums.q[first + i] = q[i];
+    }
   }
   __device__ void gather(const Command& cmd) {
     int* listed = at_rank(&sh.listed, 0);
-    u64* to = at_rank(list, 0);
+    u64* to = at_rank(sh.list, 0);
     const int shift = kOrderBits - cmd.bits;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float v = x[i];
-      if (!(v > -INFINITY)) continue;
-      const int b = scale.bucket(v);
-      if (b < cmd.first || b > cmd.last) continue;
-      const u64 o = order_of(v, lo + i);
-      if (cmd.bits && o >> shift != cmd.prefix) continue;
+    for_each(0, n, [&](float v, int i) {
+      v = seen(v);
+      const float t = scale.steps(v);
+      if (!(t >= (float)cmd.first && t < (float)(cmd.last + 1))) return;
+      const u64 o = order_of(v + 0.0f, lo + i);
+      if (cmd.bits && o >> shift != cmd.prefix) return;
       const int at = atomicAdd(listed, 1);
       if (at < kList) to[at] = o;
-    }
+    });
   }
   __device__ bool reaches_least(float v) const {
-    return exp(((double)v - (double)scale.top) / temperature) >= least || v == scale.top;
+    return exp(((double)v - (double)scale.top) / (double)temperature) >= (double)least || v == scale.top;
   }
   __device__ void count_least(const Command& cmd) {
     int* counted = at_rank(&sh.counted, 0);
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float v = x[i];
-      if (v > -INFINITY && scale.bucket(v) == cmd.first && reaches_least(v)) atomicAdd(counted, 1);
-    }
+    for_each(0, n, [&](float v, int) {
+      v = seen(v);
+      if (scale.bucket(v) == cmd.first && reaches_least(v)) atomicAdd(counted, 1);
+    });
   }
   __device__ void serve(const Command& cmd) {
     if (cmd.op == kGather) gather(cmd);
     else if (cmd.op == kCountLeast) count_least(cmd);
-    else if (cmd.op == kHistogram) {
-      clear_histogram();
-      add_up(cmd);
-    }
+    else if (cmd.op == kHistogram) add_up<true>(cmd);
   }
 
-  // ---- the leader's
+  // ---- the leader's; every thread of it takes the same way
   __device__ void ask(const Command& cmd) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = sh.counted = 0;
@@ -230,8 +310,8 @@ struct Row {
     sync_all();
   }
 
-  // The CTAs' histograms as bucket sums. `base` < 0: buckets of z; else bins inside bucket `base`, largest first.
-  __device__ void read_sums(int base, int bins) {
+  // The running sums of all CTAs. base < 0: over the buckets; else over the bins of bucket `base`, the largest first.
+  __device__ void run_sums(Running& to, int base) {
     unsigned c[kPerThread] = {};
     u64 q[kPerThread] = {};
     static_assert(kPerThread == 4, "16 bytes a thread");
@@ -239,24 +319,22 @@ struct Row {
     const int from = base < 0 ? first : kBuckets - kPerThread - first;
 #pragma unroll
     for (int r = 0; r < kCl; ++r) {
-      const unsigned* h = at_rank(hist, r);
-      const uint4 n4 = *reinterpret_cast<const uint4*>(h + from), q4 = *reinterpret_cast<const uint4*>(h + kBuckets + from);
-      const unsigned nn[4] = {n4.x, n4.y, n4.z, n4.w}, qq[4] = {q4.x, q4.y, q4.z, q4.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] += nn[base < 0 ? i : 3 - i];
-        q[i] += qq[base < 0 ? i : 3 - i];
-      }
+      const Sums* s = at_rank(&sh.sums, r);
+      const uint4 n4 = *reinterpret_cast<const uint4*>(s->count + from);
+      const ulonglong2 qa = *reinterpret_cast<const ulonglong2*>(s->q + from);
+      const ulonglong2 qb = *reinterpret_cast<const ulonglong2*>(s->q + from + 2);
+      const bool up = base < 0;
+      c[0] += up ? n4.x : n4.w, c[1] += up ? n4.y : n4.z, c[2] += up ? n4.z : n4.y, c[3] += up ? n4.w : n4.x;
+      q[0] += up ? qa.x : qb.y, q[1] += up ? qa.y : qb.x, q[2] += up ? qb.x : qa.y, q[3] += up ? qb.y : qa.x;
     }
+    double e = exp(-(double)(base < 0 ? first : base) / 64.0) * (1.0 / 8388608.0), m[kPerThread];
     unsigned tc = 0;
     double tm = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      const double e = c[i] ? exp(-(double)(base < 0 ? first + i : base) / 64.0) : 0.0;
-      count[i] = c[i];
-      mass[i] = e * ((double)(((u64)c[i] << 23) - q[i]) * (1.0 / 8388608.0));
-      tc += count[i];
-      tm += mass[i];
+      tc = c[i] += tc;
+      tm = m[i] = tm + e * (double)(((u64)(c[i] - (i ? c[i - 1] : 0)) << 23) - q[i]);
+      if (base < 0) e *= 0.98449643700540841;  // exp(-1 / 64)
     }
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     unsigned sc = tc;
@@ -270,91 +348,43 @@ struct Row {
         sm += vm;
       }
     }
-    __syncthreads();
     if (lane == 31) {
       sh.warp_count[warp] = sc;
       sh.warp_mass[warp] = sm;
     }
+    sc = __shfl_up_sync(0xffffffffu, sc, 1);
+    sm = __shfl_up_sync(0xffffffffu, sm, 1);
+    if (lane == 0) sc = 0, sm = 0.0;
     __syncthreads();
-    count_before = sc - tc;
-    mass_before = sm - tm;
-    all_count = 0;
-    all_mass = 0.0;
-    for (int w = 0; w < kWarps; ++w) {
+    unsigned wc = 0;
+    double wm = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
       if (w < warp) {
-        count_before += sh.warp_count[w];
-        mass_before += sh.warp_mass[w];
+        wc += sh.warp_count[w];
+        wm += sh.warp_mass[w];
       }
-      all_count += sh.warp_count[w];
-      all_mass += sh.warp_mass[w];
-    }
-  }
-
-  struct Found {
-    int bucket;
-    unsigned count_before, count;
-    double mass_before, mass;
-  };
-  // The first bucket that is not empty and satisfies reached(count up to its end, mass up to its end); the last one
-  // that is not empty if none does.
-  template <typename F>
-  __device__ Found find(F reached) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.found = kBuckets;
-    __syncthreads();
-    unsigned c = count_before;
-    double m = mass_before;
-    int mine = kBuckets, last = -1;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      c += count[i];
-      m += mass[i];
-      if (count[i] == 0) continue;
-      last = (int)threadIdx.x * kPerThread + i;
-      if (mine == kBuckets && reached(c, m)) mine = last;
-    }
-    if (mine < kBuckets) atomicMin(&sh.found, mine);
-    __syncthreads();
-    if (sh.found == kBuckets) {  // none (a sum's rounding): uniform over the CTA
-      __syncthreads();
-      if (threadIdx.x == 0) sh.found = -1;
-      __syncthreads();
-      if (last >= 0) atomicMax(&sh.found, last);
-      __syncthreads();
-    }
-    return at_bucket(sh.found);
-  }
-  __device__ Found at_bucket(int b) {
-    __syncthreads();
-    if ((int)threadIdx.x == b / kPerThread) {
-      unsigned c = count_before;
-      double m = mass_before;
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        if (i == b % kPerThread) {
-          sh.answer_count = c;
-          sh.answer_mass = m;
-          sh.bucket_count = count[i];
-          sh.bucket_mass = mass[i];
-        }
-        c += count[i];
-        m += mass[i];
-      }
+      to.count[first + i] = wc + sc + c[i];
+      to.mass[first + i] = wm + (sm + m[i]);
     }
     __syncthreads();
-    return {b, sh.answer_count, sh.bucket_count, sh.answer_mass, sh.bucket_mass};
   }
 
   // Sorts the gathered tokens, best first, and sums their weights: prefix[i] = sum of weights 0 .. i.
   __device__ void sort_list(int n_list) {
+    u64* list = sh.list;
     int size = 2;
     while (size < n_list) size <<= 1;
-    __syncthreads();
     for (int i = n_list + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+    // steps within 64 neighbours need only their own warp, which holds them
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
-        __syncthreads();
-        for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+        if (j >= 32 || (j == k >> 1)) __syncthreads();
+        else __syncwarp();
+        const int t = threadIdx.x;
+        if (t < size / 2) {
           const int i = 2 * t - (t & (j - 1)), p = i + j;
           const u64 u = list[i], v = list[p];
           if ((u < v) == ((i & k) == 0)) {
@@ -364,108 +394,85 @@ struct Row {
         }
       }
     __syncthreads();
-    const int i0 = 2 * threadIdx.x;
+    const int i0 = 2 * threadIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const double w0 = i0 < n_list ? scale.weight(value_of(list[i0])) : 0.0;
     const double w1 = i0 + 1 < n_list ? scale.weight(value_of(list[i0 + 1])) : 0.0;
     double s = w0 + w1;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
       const double v = __shfl_up_sync(0xffffffffu, s, i);
       if (lane >= i) s += v;
     }
     if (lane == 31) sh.warp_mass[warp] = s;
+    s = __shfl_up_sync(0xffffffffu, s, 1);
+    if (lane == 0) s = 0.0;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) s += sh.warp_mass[w];
-    if (i0 < kList) {
-      prefix[i0] = s - w1;
-      prefix[i0 + 1] = s;
-    }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (w < warp) s += sh.warp_mass[w];
+    sh.prefix[i0] = s + w0;
+    sh.prefix[i0 + 1] = s + (w0 + w1);
     __syncthreads();
   }
-  // The first place of the sorted list that satisfies reached(its number from 1, the sum with it); the last if none does.
+  // The first place of the sorted list that satisfies reached(place); the last one if none does.
   template <typename F>
-  __device__ int first_place(int n_list, F reached) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.found = n_list - 1;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_list; i += kThreads)
-      if (reached((unsigned)i + 1, prefix[i])) {
-        atomicMin(&sh.found, i);
-        break;
-      }
-    __syncthreads();
-    return sh.found;
+  __device__ int first_place(int n_list, F reached) const {
+    int a = 0, b = n_list - 1;
+    while (a < b) {
+      const int mid = (a + b) / 2;
+      if (reached(mid)) b = mid;
+      else a = mid + 1;
+    }
+    return a;
   }
 
-  // Inside bucket f: the first token for which reached(tokens, mass) holds, both counted from the bucket's first token.
-  // Leaves the sorted neighbourhood in the list. Returns the cut at that token and the token.
-  template <typename F>
-  __device__ Cut resolve(const Found& f, F reached, u64& order) {
-    Command cmd{kGather, f.bucket, f.bucket, 0, 0};
-    unsigned c0 = 0, n_in = f.count;
-    double m0 = 0.0;
-    if (n_in > kList) {
-      // crowded: narrow by digits of the order, from the top. The bucket sums make room for the bins' and return after.
-      unsigned keep_c[kPerThread + 2];
-      double keep_m[kPerThread + 2];
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        keep_c[i] = count[i];
-        keep_m[i] = mass[i];
-      }
-      keep_c[kPerThread] = count_before;
-      keep_m[kPerThread] = mass_before;
-      keep_c[kPerThread + 1] = all_count;
-      keep_m[kPerThread + 1] = all_mass;
-      while (n_in > kList) {
-        cmd.op = kHistogram;
-        ask(cmd);
-        read_sums(f.bucket, kBuckets);
-        const Found bin = find([&](unsigned c, double m) { return reached(c0 + c, m0 + m); });
-        const int digit = min(kDigit, kOrderBits - cmd.bits);
-        cmd.prefix = cmd.prefix << digit | (u64)(kBuckets - 1 - bin.bucket);
-        cmd.bits += digit;
-        c0 += bin.count_before;
-        m0 += bin.mass_before;
-        n_in = bin.count;
-      }
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        count[i] = keep_c[i];
-        mass[i] = keep_m[i];
-      }
-      count_before = keep_c[kPerThread];
-      mass_before = keep_m[kPerThread];
-      all_count = keep_c[kPerThread + 1];
-      all_mass = keep_m[kPerThread + 1];
+  // Inside bucket b: the cut at the first token with at least `need` tokens of the bucket up to it (need > 0), or a mass
+  // of everything up to it that reaches (more: exceeds) want; at most `most` tokens. Also that token.
+  __device__ Cut resolve(int b, unsigned need, double want, bool more, unsigned most, u64& order) {
+    Command cmd{kGather, b, b, 0, 0};
+    unsigned c0 = 0, n_in = sh.row.count[b] - sh.row.before(b);
+    double m0 = sh.row.mass_before(b);
+    most = min(most, n_in);
+    while (n_in > kList) {  // crowded: narrow by digits of the order, from the top
+      cmd.op = kHistogram;
+      ask(cmd);
+      run_sums(sh.bins, b);
+      int bin = need ? sh.bins.find_count(need - c0) : sh.bins.find_mass(want - m0, more);
+      bin = min(bin, sh.bins.find_count(most - c0));
+      const int digit = min(kDigit, kOrderBits - cmd.bits);
+      cmd.prefix = cmd.prefix << digit | (u64)(kBuckets - 1 - bin);
+      cmd.bits += digit;
+      n_in = sh.bins.count[bin] - sh.bins.before(bin);
+      c0 += sh.bins.before(bin);
+      m0 += sh.bins.mass_before(bin);
       cmd.op = kGather;
     }
     ask(cmd);
     sort_list((int)n_in);
-    const int at = first_place((int)n_in, [&](unsigned c, double m) { return reached(c0 + c, m0 + m); });
-    order = list[at];
-    const Cut cut{f.bucket, c0 + at + 1, f.mass_before + m0 + prefix[at]};
-    __syncthreads();
-    return cut;
+    const int at = first_place(min(n_in, most - c0), [&](int i) {
+      return need ? c0 + i + 1 >= need : (more ? m0 + sh.prefix[i] > want : m0 + sh.prefix[i] >= want);
+    });
+    order = sh.list[at];
+    return {b, c0 + at + 1, m0 + sh.prefix[at]};
   }
 
-  __device__ void lead(float u, int k, float p, float mp, u64 best, u64& order, double& total) {
-    read_sums(-1, kBuckets);
-    bool use_p = p < 1.0f, use_least = mp > 0.0f;
-    if ((use_p && p <= 0.0f) || mp > 1.0f) k = 1;
+  __device__ void lead(float u, int k, float p, u64 best, u64& order, double& total) {
+    bool use_p = p < 1.0f, use_least = least > 0.0f;
+    if ((use_p && p <= 0.0f) || least > 1.0f) k = 1;
     if (k == 1) {
       order = best;
       total = 1.0;
       return;
     }
-    if (k < 0 || (unsigned)k >= all_count) k = 0;
+    run_sums(sh.row, -1);
+    const Running& row = sh.row;
+    const unsigned all = row.count[kBuckets - 1];
+    if (k < 0 || (unsigned)k >= all) k = 0;
     int least_bucket = kBuckets;
     if (use_least) {
-      least = mp;
-      const double z = -log((double)mp) * 64.0;
+      const double z = -log((double)least) * 64.0;
       use_least = z < kBuckets;
-      least_bucket = use_least ? max(0, (int)z) : kBuckets;
+      if (use_least) least_bucket = max(0, (int)z);
     }
     const double draw = u > 0.0f ? (double)u : 0.0;
 
@@ -473,68 +480,59 @@ struct Row {
     // needs the sum of all that top_k keeps
     if (k || use_p || use_least) {
       int bound = kBuckets - 1;
-      if (k) bound = find([&](unsigned c, double) { return c >= (unsigned)k; }).bucket;
-      else if (use_p) bound = find([&](unsigned, double m) { return m >= (double)p * all_mass; }).bucket;
+      if (k) bound = row.find_count(k);
+      else if (use_p) bound = row.find_mass((double)p * row.mass[kBuckets - 1], false);
       if (use_least && !(k && use_p)) bound = min(bound, least_bucket);
-      const Found f = at_bucket(bound);
-      const unsigned n_in = f.count_before + f.count;
-      if (n_in <= kList) {
-        // few: sort them all and filter there
+      const int n_in = (int)row.count[bound];
+      if (n_in <= kList) {  // few: sort them all and filter there
         ask({kGather, 0, bound, 0, 0});
-        sort_list((int)n_in);
-        int kept = k ? min(k, (int)n_in) : (int)n_in;
+        sort_list(n_in);
+        int kept = k ? min(k, n_in) : n_in;
         if (use_p) {
           // without top_k the whole sum counts, behind the bound too
-          const double want = (double)p * (k ? prefix[kept - 1] : all_mass);
-          kept = min(kept, 1 + first_place((int)n_in, [&](unsigned, double m) { return m >= want; }));
+          const double want = (double)p * (k ? sh.prefix[kept - 1] : row.mass[kBuckets - 1]);
+          kept = 1 + first_place(kept, [&](int i) { return sh.prefix[i] >= want; });
         }
         if (use_least) {
-          const int out = first_place((int)n_in, [&](unsigned c, double) { return !reaches_least(value_of(list[c - 1])); });
-          if (!reaches_least(value_of(list[out]))) kept = min(kept, max(1, out));
+          const int out = first_place(kept, [&](int i) { return !reaches_least(value_of(sh.list[i])); });
+          if (!reaches_least(value_of(sh.list[out]))) kept = max(1, out);
         }
-        total = prefix[kept - 1];
+        total = sh.prefix[kept - 1];
         const double want = draw * total;
-        const int at = min(kept - 1, first_place((int)n_in, [&](unsigned, double m) { return m > want; }));
-        order = list[at];
+        order = sh.list[first_place(kept, [&](int i) { return sh.prefix[i] > want; })];
         return;
       }
     }
 
-    Cut cut{kBuckets, 0, all_mass};  // nothing is cut off
+    Cut cut{kBuckets, 0, row.mass[kBuckets - 1]};  // nothing is cut off
     if (k) {
-      const Found f = find([&](unsigned c, double) { return c >= (unsigned)k; });
-      const unsigned in = (unsigned)k - f.count_before;
-      if (in == f.count) cut = {f.bucket, in, f.mass_before + f.mass};
-      else cut = resolve(f, [&](unsigned c, double) { return c >= in; }, order);
+      const int b = row.find_count(k);
+      if (row.count[b] == (unsigned)k) cut = {b, (unsigned)k - row.before(b), row.mass[b]};
+      else cut = resolve(b, (unsigned)k - row.before(b), 0.0, false, ~0u, order);
     }
     if (use_p) {
       const double want = (double)p * cut.mass;
-      const Found f = find([&](unsigned, double m) { return m >= want; });
-      if (f.bucket <= cut.bucket) {
-        const Cut by_p = resolve(f, [&](unsigned, double m) { return f.mass_before + m >= want; }, order);
-        if (f.bucket < cut.bucket || by_p.count < cut.count) cut = by_p;
-      }
+      const int b = row.find_mass(want, false);
+      if (b < cut.bucket || (b == cut.bucket && cut.count > 0)) cut = resolve(b, 0, want, false, b < cut.bucket ? ~0u : cut.count, order);
     }
     if (use_least && least_bucket <= cut.bucket) {
-      const Found f = at_bucket(least_bucket);
       ask({kCountLeast, least_bucket, least_bucket, 0, 0});
-      const unsigned in = (unsigned)sh.counted;
+      const unsigned in = (unsigned)sh.counted, has = row.count[least_bucket] - row.before(least_bucket);
       if (least_bucket < cut.bucket || in < cut.count) {
-        if (in == 0) cut = {least_bucket, 0, f.mass_before};
-        else if (in == f.count) cut = {least_bucket, in, f.mass_before + f.mass};
-        else cut = resolve(f, [&](unsigned c, double) { return c >= in; }, order);
+        if (in == 0) cut = {least_bucket, 0, row.mass_before(least_bucket)};
+        else if (in == has) cut = {least_bucket, in, row.mass[least_bucket]};
+        else cut = resolve(least_bucket, in, 0.0, false, ~0u, order);
       }
     }
     total = cut.mass;
     const double want = draw * total;
-    const Found f = find([&](unsigned, double m) { return m > want; });
-    if (f.bucket < cut.bucket || (f.bucket == cut.bucket && cut.count > 0)) {
-      const unsigned most = f.bucket < cut.bucket ? f.count : cut.count;
-      resolve(f, [&](unsigned c, double m) { return c >= most || f.mass_before + m > want; }, order);
+    int b = row.find_mass(want, true);
+    if (b < cut.bucket || (b == cut.bucket && cut.count > 0)) {
+      resolve(b, 0, want, true, b < cut.bucket ? ~0u : cut.count, order);
     } else {  // the draw fell behind the cut by a rounding: the last one kept
-      const unsigned kept = at_bucket(cut.bucket).count_before + cut.count;
-      const Found g = find([&](unsigned c, double) { return c >= kept; });
-      resolve(g, [&](unsigned c, double) { return g.count_before + c >= kept; }, order);
+      const unsigned kept = row.before(cut.bucket) + cut.count;
+      b = row.find_count(kept);
+      resolve(b, kept - row.before(b), 0.0, false, ~0u, order);
     }
   }
 };
@@ -542,53 +540,31 @@ struct Row {
 template <int kType, int kCl>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice) {
   using R = Row<kType, kCl>;
-  using T = typename R::T;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ Shared sh;
-  const int row = blockIdx.x / kCl, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  R r(a, sh);
-  r.rank = blockIdx.x % kCl;
-  r.hist = reinterpret_cast<unsigned*>(smem);
-  r.list = reinterpret_cast<u64*>(smem);
-  r.prefix = reinterpret_cast<double*>(smem) + kList;
-  r.x = reinterpret_cast<float*>(smem + 2 * kBuckets * 4);
-  r.lo = min(a.vocab, r.rank * slice);
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  const int row = blockIdx.x / kCl, rank = blockIdx.x % kCl, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  R r(sh);
+  r.lo = min(a.vocab, rank * slice);
   r.n = min(slice, a.vocab - r.lo);
+  r.x = static_cast<const typename R::T*>(a.logits) + (long long)row * a.stride + r.lo;
 
-  // the logits, and the best of them
-  const T* from = static_cast<const T*>(a.logits) + (long long)row * a.stride + r.lo;
   float top = -INFINITY;
   int top_at = 0;
-  auto take = [&](int i, float v) {
-    v = v == v ? v + 0.0f : -INFINITY;  // -0 becomes +0: they tie
-    r.x[i] = v;
-    if (v > top) {
+  r.for_each(0, r.n, [&](float v, int i) {
+    if (v > top || (v == top && i < top_at)) {  // never for NaN
       top = v;
       top_at = i;
     }
-  };
-  constexpr int kVec = 16 / (int)sizeof(T);
-  int i = 0;
-  if (reinterpret_cast<uintptr_t>(from) % 16 == 0) {
-    const int whole = r.n / kVec;
-#pragma unroll 4
-    for (int v = threadIdx.x; v < whole; v += kThreads) {
-      const uint4 b = __ldg(reinterpret_cast<const uint4*>(from) + v);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) take(v * kVec + e, to_float(reinterpret_cast<const T*>(&b)[e]));
-    }
-    i = whole * kVec;
-  }
-#pragma unroll 8
-  for (i += threadIdx.x; i < r.n; i += kThreads) take(i, to_float(from[i]));
-  u64 best = top > -INFINITY ? order_of(top, r.lo + top_at) : 0;
+  });
+  u64 best = top > -INFINITY ? order_of(top + 0.0f, r.lo + top_at) : 0;  // -0 becomes +0: they tie
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, s));
   if (lane == 0) sh.warp_best[warp] = best;
-  r.clear_histogram();  // ends with a barrier
+  __syncthreads();
   if (threadIdx.x < kCl) {
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) best = max(best, sh.warp_best[w]);
-    r.at_rank(sh.best, threadIdx.x)[r.rank] = best;
+    r.at_rank(sh.best, threadIdx.x)[rank] = best;
   }
   r.sync_all();
   best = 0;
@@ -597,26 +573,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice
 
   const float t = a.temperature ? __ldg(a.temperature + row) : 1.0f;
   if (best == 0 || !(t >= 1.17549435e-38f)) {
-    if (r.rank == 0 && threadIdx.x == 0) {
+    if (rank == 0 && threadIdx.x == 0) {
       a.tokens[row] = best == 0 ? -1 : index_of(best);
       if (a.probs) a.probs[row] = best == 0 ? 0.0f : 1.0f;
     }
     return;
   }
-  r.scale = Scale(value_of(best), t);
+  r.top_infinite = value_of(best) == INFINITY;
+  r.scale = Scale(r.seen(value_of(best)), t);
   r.temperature = t;
-  const float mp = a.min_p ? __ldg(a.min_p + row) : 0.0f;
-  r.least = mp;
-  r.add_up({kHistogram, 0, kBuckets - 1, 0, 0});
+  r.least = a.min_p ? __ldg(a.min_p + row) : 0.0f;
+  r.template add_up<false>({kHistogram, 0, kBuckets - 1, 0, 0});
   r.sync_all();
-  if (r.rank == 0) {
+  if (rank == 0) {
     u64 order = best;
     double total = 1.0;
-    r.lead(__ldg(a.uniforms + row), a.top_k ? __ldg(a.top_k + row) : 0, a.top_p ? __ldg(a.top_p + row) : 1.0f, mp, best, order,
-           total);
+    r.lead(__ldg(a.uniforms + row), a.top_k ? __ldg(a.top_k + row) : 0, a.top_p ? __ldg(a.top_p + row) : 1.0f, best, order, total);
     if (threadIdx.x == 0) {
       a.tokens[row] = index_of(order);
-      if (a.probs) a.probs[row] = (float)(r.scale.weight(value_of(order)) / total);
+      // the best token may be +infinity, which the sums see as 0; its weight is 1 in any case
+      if (a.probs) a.probs[row] = order == best ? (float)(1.0 / total) : (float)(r.scale.weight(value_of(order)) / total);
     }
     if (kCl > 1) r.ask({kDone, 0, 0, 0, 0});
   } else {
@@ -633,13 +609,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice
 template <int kType, int kCl>
 cudaError_t launch(const Sample& a, cudaStream_t s) {
   const int slice = ((a.vocab + kCl - 1) / kCl + 15) / 16 * 16;
-  const int smem = 2 * kBuckets * 4 + slice * 4;
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<kType, kCl>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<kType, kCl>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * kCl);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -652,7 +627,9 @@ cudaError_t launch(const Sample& a, cudaStream_t s) {
 
 template <int kType>
 cudaError_t launch(const Sample& a, cudaStream_t s) {
-  return a.vocab <= kOneCta ? launch<kType, 1>(a, s) : launch<kType, kCluster>(a, s);
+  if (a.vocab <= kOneCta || a.rows * 2 > kResident) return launch<kType, 1>(a, s);
+  if (a.rows * 4 > kResident) return launch<kType, 2>(a, s);
+  return a.rows * 8 > kResident ? launch<kType, 4>(a, s) : launch<kType, 8>(a, s);
 }
 
 }  // namespace
