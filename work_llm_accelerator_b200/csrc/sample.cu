@@ -39,29 +39,51 @@ constexpr int kList = 1024;  // tokens that are sorted at once
 constexpr int kOrderBits = 50;
 constexpr int kDigit = 11;        // bits by which a crowded bucket is narrowed at a time
 constexpr int kFold = 1 << 15;    // logits whose q, below 2^17 each, fit a 32-bit sum
+constexpr int kLight = 8;         // 16-byte loads that a thread has under way in the passes that only compare
+constexpr int kHeavy = 4;         // and in the pass that sums
 constexpr int kMaxCluster = 8;
 constexpr int kOneCta = 8192;     // vocabularies up to this size take one CTA: less to read than a cluster costs to sync
 constexpr int kResident = 2 * 148;  // CTAs that fit the GPU at once
 
 typedef unsigned long long u64;
 
+// A type's values: one from memory, and the kVec ones of 16 bytes (by bit operations, so that they stay in registers).
 template <int kType>
 struct TypeOf;
 template <>
 struct TypeOf<0> {
   using T = float;
+  static constexpr int kVec = 4;
+  static __device__ __forceinline__ float one(const T* p) { return __ldg(p); }
+  static __device__ __forceinline__ void unpack(const uint4& b, float (&v)[kVec]) {
+    v[0] = __uint_as_float(b.x), v[1] = __uint_as_float(b.y), v[2] = __uint_as_float(b.z), v[3] = __uint_as_float(b.w);
+  }
 };
 template <>
 struct TypeOf<1> {
   using T = __half;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float one(const T* p) { return __half2float(*p); }
+  static __device__ __forceinline__ float half_at(unsigned w, int hi) {
+    return __half2float(__ushort_as_half((unsigned short)(hi ? w >> 16 : w & 0xffffu)));
+  }
+  static __device__ __forceinline__ void unpack(const uint4& b, float (&v)[kVec]) {
+    v[0] = half_at(b.x, 0), v[1] = half_at(b.x, 1), v[2] = half_at(b.y, 0), v[3] = half_at(b.y, 1);
+    v[4] = half_at(b.z, 0), v[5] = half_at(b.z, 1), v[6] = half_at(b.w, 0), v[7] = half_at(b.w, 1);
+  }
 };
 template <>
 struct TypeOf<2> {
   using T = __nv_bfloat16;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float one(const T* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void unpack(const uint4& b, float (&v)[kVec]) {
+    v[0] = __uint_as_float(b.x << 16), v[1] = __uint_as_float(b.x & 0xffff0000u);
+    v[2] = __uint_as_float(b.y << 16), v[3] = __uint_as_float(b.y & 0xffff0000u);
+    v[4] = __uint_as_float(b.z << 16), v[5] = __uint_as_float(b.z & 0xffff0000u);
+    v[6] = __uint_as_float(b.w << 16), v[7] = __uint_as_float(b.w & 0xffff0000u);
+  }
 };
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 __device__ __forceinline__ unsigned key_of(float x) {
   const unsigned b = __float_as_uint(x);
@@ -74,8 +96,36 @@ __device__ __forceinline__ u64 order_of(float x, int i) { return (u64)key_of(x) 
 __device__ __forceinline__ int index_of(u64 order) { return kMaxVocab - 1 - (int)(order & (kMaxVocab - 1)); }
 __device__ __forceinline__ float value_of(u64 order) { return value_of((unsigned)(order >> 18)); }
 
-// 64 z = 64 (top - x) / temperature in parts: bucket and q. The product with 64 / temperature = c + c_low is exact to
-// about 2^-48, and so is its distance to the bucket's border.
+// Pairs of fp32 numbers in one instruction.
+typedef u64 F2;
+__device__ __forceinline__ F2 pair(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add2_down(F2 a, F2 b) {
+  F2 r;
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 64 z = 64 (top - x) / temperature in parts: bucket and q. 64 / temperature = c + c_low to 2^-48, so that no error is
+// common to all weights; the difference top - x is rounded to fp32.
 struct Scale {
   float top, c, c_low;
   __device__ Scale() {}
@@ -86,6 +136,14 @@ struct Scale {
     c = fminf(64.0f * r, 3.4028235e38f);  // finite, so that the best token stays at 0 steps
     c_low = 64.0f * low;
   }
+  static constexpr float kFloor = 8388608.0f;  // 2^23: added rounding down, the sum's low bits are the floor
+  // q + kQBits as bits: the conversion is the addition of 1.5 * 2^23. The 64 keeps a q of -12 positive, which the
+  // rounding of a step count next to its bucket's border can give.
+  static constexpr float kRound = 12582912.0f + 64.0f;
+  static constexpr unsigned kQBits = 0x4b400000u + 64u;
+  // 2^23 (1 - exp(-f / 64)) = k1 f + k2 f^2 + k3 f^3 + k4 f^4, the next term below 2^-36 of it
+  static constexpr float k1 = 131072.0f, k2 = -1024.0f, k3 = 16.0f / 3.0f, k4 = -1.0f / 48.0f;
+
   __device__ __forceinline__ float steps(float x) const { return (top - x) * c; }
   static __device__ __forceinline__ bool counts(float steps) { return steps < (float)kBuckets; }  // false for NaN
   // the bucket, or -1 for a weight that counts as 0
@@ -93,21 +151,28 @@ struct Scale {
     const float t = steps(x);
     return counts(t) ? (int)t : -1;
   }
-  // q + kQBits, for a logit in bucket b (both conversions by adding 1.5 * 2^23, not on the slow pipe)
-  static constexpr unsigned kQBits = 0x4b400000u;
   __device__ __forceinline__ unsigned part_bits(float x, float b) const {
-    const float d = top - x, s = top - d;
-    const float low = (top - (s + d)) - (x - s);  // d + low is top - x exactly (two-sum)
-    float f = fmaf(d, c, -b) + fmaf(d, c_low, low * c);
-    f = fminf(fmaxf(f, 0.0f), 1.0f);
-    // 2^23 (1 - exp(-f / 64)); the series' next term is below 2^-36
-    constexpr float k1 = 131072.0f, k2 = -1024.0f, k3 = 16.0f / 3.0f, k4 = -1.0f / 48.0f;
-    return __float_as_uint(fmaf(f, fmaf(f, fmaf(f, fmaf(f, k4, k3), k2), k1), 12582912.0f));
+    const float d = top - x, f = fmaf(d, c_low, fmaf(d, c, -b));
+    return __float_as_uint(fmaf(f, fmaf(f, fmaf(f, fmaf(f, k4, k3), k2), k1), kRound));
+  }
+  // The same for two logits: bucket (in the low bits of `up`) and q.
+  __device__ __forceinline__ void two(float x, float y, float2& steps, float2& up, float2& q) const {
+    const F2 minus = pair(-1.0f, -1.0f), tops = pair(top, top), cs = pair(c, c);
+    const F2 d = fma2(pair(x, y), minus, tops), t = mul2(d, cs), u = add2_down(t, pair(kFloor, kFloor));
+    F2 f = fma2(u, minus, pair(kFloor, kFloor));  // - floor
+    f = fma2(d, pair(c_low, c_low), fma2(d, cs, f));
+    F2 e = fma2(f, pair(k4, k4), pair(k3, k3));
+    e = fma2(f, e, pair(k2, k2));
+    e = fma2(f, e, pair(k1, k1));
+    q = unpair(fma2(f, e, pair(kRound, kRound)));
+    steps = unpair(t);
+    up = unpair(u);
   }
   // the weight in 64 bits, as the sums have it
   __device__ double weight(float x) const {
     const int b = bucket(x);
-    return b < 0 ? 0.0 : exp(-(double)b / 64.0) * (double)(8388608u - (part_bits(x, (float)b) - kQBits)) * (1.0 / 8388608.0);
+    return b < 0 ? 0.0
+                 : exp(-(double)b / 64.0) * (double)(8388608 - (int)(part_bits(x, (float)b) - kQBits)) * (1.0 / 8388608.0);
   }
 };
 
@@ -121,7 +186,7 @@ struct Command {
 
 struct Sums {
   unsigned count[kBuckets];
-  u64 q[kBuckets];
+  u64 q[kBuckets];  // signed sums
 };
 // Running sums up to and with each bucket.
 struct Running {
@@ -159,7 +224,8 @@ struct Shared {
     };
   };
   Sums sums;       // this CTA's
-  Running row;     // the leader's: of all CTAs
+  Sums total;      // the leader's: of all CTAs
+  Running row;     // the leader's: over the buckets
   Running bins;    // the leader's: of the bins of a crowded bucket, best first
   u64 best[kMaxCluster];
   Command command;
@@ -178,7 +244,8 @@ struct Cut {
 
 template <int kType, int kCl>
 struct Row {
-  using T = typename TypeOf<kType>::T;
+  using V = TypeOf<kType>;
+  using T = typename V::T;
   Shared& sh;
   const T* x;  // this CTA's logits
   int lo, n;   // the first one's index, their number
@@ -198,28 +265,39 @@ struct Row {
     return p;
   }
 
-  // f(logit, its place in x) for places from .. to - 1 of this CTA's logits: 16-byte loads, four at a time, between the
-  // first and the last aligned place.
-  template <typename F>
+  // f(values, number of them, place of the first) for places from .. to - 1 of this CTA's logits: 16-byte loads, a few
+  // at a time, between the first and the last aligned place, single ones outside.
+  template <int kAhead, typename F>
   __device__ __forceinline__ void for_each(int from, int to, F f) {
-    constexpr int kVec = 16 / (int)sizeof(T), kAhead = 4;
+    constexpr int kVec = V::kVec;
     const int head = min(to - from, (int)((16 - reinterpret_cast<uintptr_t>(x + from) % 16) % 16 / sizeof(T)));
     const int vecs = (to - from - head) / kVec, tail = from + head + vecs * kVec;
-    if ((int)threadIdx.x < head) f(to_float(x[from + threadIdx.x]), from + (int)threadIdx.x);
-    if ((int)threadIdx.x < to - tail) f(to_float(x[tail + threadIdx.x]), tail + (int)threadIdx.x);
-    const uint4* v = reinterpret_cast<const uint4*>(x + from + head);
-    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kAhead) {
+    if ((int)threadIdx.x < head + (to - tail)) {
+      const int at = (int)threadIdx.x < head ? from + (int)threadIdx.x : tail + (int)threadIdx.x - head;
+      const float e[1] = {V::one(x + at)};
+      f(e, at);
+    }
+    const uint4* v = reinterpret_cast<const uint4*>(x + from + head) + threadIdx.x;
+    int at = from + head + (int)threadIdx.x * kVec, left = vecs - (int)threadIdx.x;
+    for (; left > (kAhead - 1) * kThreads; left -= kAhead * kThreads) {
       uint4 b[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (i0 + k * kThreads < vecs) b[k] = __ldg(v + i0 + k * kThreads);
+      for (int k = 0; k < kAhead; ++k) b[k] = __ldg(v + k * kThreads);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (i0 + k * kThreads >= vecs) break;
-#pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          f(to_float(reinterpret_cast<const T*>(&b[k])[e]), from + head + (i0 + k * kThreads) * kVec + e);
+        float e[kVec];
+        V::unpack(b[k], e);
+        f(e, at + k * kThreads * kVec);
       }
+      v += kAhead * kThreads;
+      at += kAhead * kThreads * kVec;
+    }
+    for (; left > 0; left -= kThreads) {
+      float e[kVec];
+      V::unpack(__ldg(v), e);
+      f(e, at);
+      v += kThreads;
+      at += kThreads * kVec;
     }
   }
   // a logit as the sums see it: where the largest is +infinity, one of 0 and nothing beside it
@@ -230,6 +308,10 @@ struct Row {
     for (int i = threadIdx.x; i < 2 * kBuckets; i += kThreads) sh.hist[0][i] = 0;
     __syncthreads();
   }
+  static __device__ __forceinline__ void count_one(unsigned address, unsigned q) {
+    asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(address) : "memory");
+    asm volatile("red.shared.add.u32 [%0 + %2], %1;" ::"r"(address), "r"(q), "n"(kBuckets * 4) : "memory");
+  }
   // Counts and q of every bucket, or of the bins of one bucket, into sh.sums.
   template <bool kBins>
   __device__ void add_up(const Command& cmd) {
@@ -237,29 +319,51 @@ struct Row {
     u64 q[kPerThread] = {};
     const int shift = kOrderBits - cmd.bits, digit = min(kDigit, shift);
     const int first = threadIdx.x * kPerThread;
+    const unsigned hist = (unsigned)__cvta_generic_to_shared(&sh.hist[0][0]) - 4 * __float_as_uint(Scale::kFloor);
     for (int from = 0; from < max(n, 1); from += kFold) {
       clear_histogram();
-      for_each(from, min(n, from + kFold), [&](float v, int i) {
-        v = seen(v);
-        const float t = scale.steps(v);
-        if (!Scale::counts(t)) return;
-        const float up = __fadd_rd(t, 8388608.0f);  // floor(t) in the low bits
-        const int b = __float_as_uint(up) & (2 * kBuckets - 1);
-        int bin = b;
-        if (kBins) {
-          const u64 o = order_of(v + 0.0f, lo + i);
-          if (b != cmd.first || (cmd.bits && o >> shift != cmd.prefix)) return;
-          bin = (int)(o >> (shift - digit)) & ((1 << digit) - 1);
+      for_each<kHeavy>(from, min(n, from + kFold), [&](const auto& e, int at) {
+        constexpr int kN = (int)(sizeof(e) / sizeof(float));
+        float v[kN];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = e[i];
+        if (top_infinite) {
+#pragma unroll
+          for (int i = 0; i < kN; ++i) v[i] = seen(v[i]);
         }
-        atomicAdd(&sh.hist[0][bin], 1u);
-        atomicAdd(&sh.hist[1][bin], scale.part_bits(v, up - 8388608.0f));
+        if (kBins || kN == 1) {
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const int b = scale.bucket(v[i]);
+            if (b < 0) continue;
+            int bin = b;
+            if (kBins) {
+              const u64 o = order_of(v[i] + 0.0f, lo + at + i);
+              if (b != cmd.first || (cmd.bits && o >> shift != cmd.prefix)) continue;
+              bin = (int)(o >> (shift - digit)) & ((1 << digit) - 1);
+            }
+            atomicAdd(&sh.hist[0][bin], 1u);
+            atomicAdd(&sh.hist[1][bin], scale.part_bits(v[i], (float)b));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i + 1 < kN; i += 2) {
+            float2 t, up, q;
+            scale.two(v[i], v[i + 1], t, up, q);
+            // 4 * (bits of up) is 4 * bucket and a constant that goes into the address
+            const unsigned a0 = hist + 4 * __float_as_uint(up.x), a1 = hist + 4 * __float_as_uint(up.y);
+            if (Scale::counts(t.x)) count_one(a0, __float_as_uint(q.x));
+            if (Scale::counts(t.y)) count_one(a1, __float_as_uint(q.y));
+          }
+        }
       });
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < kPerThread; ++i) {
         const unsigned k = sh.hist[0][first + i];
         c[i] += k;
-        q[i] += sh.hist[1][first + i] - k * Scale::kQBits;  // modulo 2^32, which the sum of q is below
+        // modulo 2^32 the sum of q + 64, which is positive and below 2^32
+        q[i] += (u64)(sh.hist[1][first + i] - k * (Scale::kQBits - 64u)) - 64ull * k;
       }
       __syncthreads();
     }
@@ -273,14 +377,25 @@ struct Row {
     int* listed = at_rank(&sh.listed, 0);
     u64* to = at_rank(sh.list, 0);
     const int shift = kOrderBits - cmd.bits;
-    for_each(0, n, [&](float v, int i) {
-      v = seen(v);
-      const float t = scale.steps(v);
-      if (!(t >= (float)cmd.first && t < (float)(cmd.last + 1))) return;
-      const u64 o = order_of(v + 0.0f, lo + i);
-      if (cmd.bits && o >> shift != cmd.prefix) return;
-      const int at = atomicAdd(listed, 1);
-      if (at < kList) to[at] = o;
+    // An interval that holds the logits of those buckets, a little wider: two comparisons settle almost every logit.
+    const float a = scale.top - (float)(cmd.last + 1) / scale.c, b = scale.top - (float)cmd.first / scale.c;
+    const float wide = (fabsf(scale.top) + fmaxf(fabsf(a), fabsf(b))) * 1e-6f;
+    const float v_low = a - wide, v_high = b + wide;  // NaN or infinite: every logit is looked at
+    for_each<kLight>(0, n, [&](const auto& e, int at) {
+      constexpr int kN = (int)(sizeof(e) / sizeof(float));
+      bool any = top_infinite;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) any = any || !(e[i] < v_low || e[i] > v_high);
+      if (!any) return;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float v = seen(e[i]), t = scale.steps(v);
+        if (!(t >= (float)cmd.first && t < (float)(cmd.last + 1))) continue;
+        const u64 o = order_of(v + 0.0f, lo + at + i);
+        if (cmd.bits && o >> shift != cmd.prefix) continue;
+        const int place = atomicAdd(listed, 1);
+        if (place < kList) to[place] = o;
+      }
     });
   }
   __device__ bool reaches_least(float v) const {
@@ -288,15 +403,21 @@ struct Row {
   }
   __device__ void count_least(const Command& cmd) {
     int* counted = at_rank(&sh.counted, 0);
-    for_each(0, n, [&](float v, int) {
-      v = seen(v);
-      if (scale.bucket(v) == cmd.first && reaches_least(v)) atomicAdd(counted, 1);
+    for_each<1>(0, n, [&](const auto& e, int) {
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(e) / sizeof(float)); ++i) {
+        const float v = seen(e[i]);
+        if (scale.bucket(v) == cmd.first && reaches_least(v)) atomicAdd(counted, 1);
+      }
     });
   }
   __device__ void serve(const Command& cmd) {
     if (cmd.op == kGather) gather(cmd);
     else if (cmd.op == kCountLeast) count_least(cmd);
-    else if (cmd.op == kHistogram) add_up<true>(cmd);
+    else if (cmd.op == kHistogram) {
+      add_up<true>(cmd);
+      share_sums();
+    }
   }
 
   // ---- the leader's; every thread of it takes the same way
@@ -310,22 +431,48 @@ struct Row {
     sync_all();
   }
 
+  // The CTAs' sums into the leader's: each adds an eighth of the buckets over all of them. Ends with all CTAs in step.
+  __device__ void share_sums() {
+    sync_all();
+    if (kCl == 1) return;
+    constexpr int kEach = kBuckets / kCl, kLanes = kThreads / kEach;  // threads per bucket
+    constexpr int kTurns = kLanes ? 1 : kEach / kThreads, kSplit = kLanes ? kLanes : 1;
+    const int rank = (int)cg::this_cluster().block_rank();
+#pragma unroll
+    for (int turn = 0; turn < kTurns; ++turn) {
+      const int b = rank * kEach + turn * kThreads + (int)threadIdx.x / kSplit, part = threadIdx.x % kSplit;
+      unsigned c = 0;
+      u64 q = 0;
+#pragma unroll
+      for (int r = 0; r < kCl / kSplit; ++r) {
+        const Sums* s = at_rank(&sh.sums, r * kSplit + part);
+        c += s->count[b];
+        q += s->q[b];
+      }
+#pragma unroll
+      for (int i = 1; i < kSplit; i <<= 1) {
+        c += __shfl_xor_sync(0xffffffffu, c, i);
+        q += __shfl_xor_sync(0xffffffffu, q, i);
+      }
+      if (part == 0) {
+        at_rank(&sh.total, 0)->count[b] = c;
+        at_rank(&sh.total, 0)->q[b] = q;
+      }
+    }
+    sync_all();
+  }
   // The running sums of all CTAs. base < 0: over the buckets; else over the bins of bucket `base`, the largest first.
   __device__ void run_sums(Running& to, int base) {
-    unsigned c[kPerThread] = {};
-    u64 q[kPerThread] = {};
     static_assert(kPerThread == 4, "16 bytes a thread");
     const int first = threadIdx.x * kPerThread;
     const int from = base < 0 ? first : kBuckets - kPerThread - first;
+    const Sums& s = kCl == 1 ? sh.sums : sh.total;
+    unsigned c[kPerThread];
+    u64 q[kPerThread];
 #pragma unroll
-    for (int r = 0; r < kCl; ++r) {
-      const Sums* s = at_rank(&sh.sums, r);
-      const uint4 n4 = *reinterpret_cast<const uint4*>(s->count + from);
-      const ulonglong2 qa = *reinterpret_cast<const ulonglong2*>(s->q + from);
-      const ulonglong2 qb = *reinterpret_cast<const ulonglong2*>(s->q + from + 2);
-      const bool up = base < 0;
-      c[0] += up ? n4.x : n4.w, c[1] += up ? n4.y : n4.z, c[2] += up ? n4.z : n4.y, c[3] += up ? n4.w : n4.x;
-      q[0] += up ? qa.x : qb.y, q[1] += up ? qa.y : qb.x, q[2] += up ? qb.x : qa.y, q[3] += up ? qb.y : qa.x;
+    for (int i = 0; i < kPerThread; ++i) {
+      c[i] = s.count[from + (base < 0 ? i : kPerThread - 1 - i)];
+      q[i] = s.q[from + (base < 0 ? i : kPerThread - 1 - i)];
     }
     double e = exp(-(double)(base < 0 ? first : base) / 64.0) * (1.0 / 8388608.0), m[kPerThread];
     unsigned tc = 0;
@@ -333,7 +480,7 @@ struct Row {
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       tc = c[i] += tc;
-      tm = m[i] = tm + e * (double)(((u64)(c[i] - (i ? c[i - 1] : 0)) << 23) - q[i]);
+      tm = m[i] = tm + e * (double)(long long)(((u64)(c[i] - (i ? c[i - 1] : 0)) << 23) - q[i]);
       if (base < 0) e *= 0.98449643700540841;  // exp(-1 / 64)
     }
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -550,12 +697,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice
 
   float top = -INFINITY;
   int top_at = 0;
-  r.for_each(0, r.n, [&](float v, int i) {
-    if (v > top || (v == top && i < top_at)) {  // never for NaN
-      top = v;
-      top_at = i;
+  r.template for_each<kLight>(0, r.n, [&](const auto& e, int at) {
+    float m = e[0];
+#pragma unroll
+    for (int i = 1; i < (int)(sizeof(e) / sizeof(float)); ++i) m = fmaxf(m, e[i]);
+    if (m > top || (m == top && at < top_at)) {  // never for NaN
+      top = m;
+      top_at = at;
     }
   });
+  // the place of the group's first such value
+  while (top > -INFINITY && R::V::one(r.x + top_at) != top) ++top_at;
   u64 best = top > -INFINITY ? order_of(top + 0.0f, r.lo + top_at) : 0;  // -0 becomes +0: they tie
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, s));
@@ -584,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice
   r.temperature = t;
   r.least = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   r.template add_up<false>({kHistogram, 0, kBuckets - 1, 0, 0});
-  r.sync_all();
+  r.share_sums();
   if (rank == 0) {
     u64 order = best;
     double total = 1.0;
