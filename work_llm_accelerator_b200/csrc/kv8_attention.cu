@@ -2,22 +2,28 @@
 // own length, softmax in one pass with the running maximum and sum in fp32.
 //
 // Mathematics. With k_j = s_k c_j and v_j = s_v d_j (int8 codes, one scale per 64-token block) a score is
-// (scale s_k) (q . c_j), and a tile of 32 tokens adds s_v sum_j p_j d_j: both products run on the codes, on
-// mma.sync m16n8k16 in fp16, where a code is exact, and the scales multiply fp32 sums. q and the weights p would
-// lose 13 bits in fp16, so each is the sum of two fp16 numbers, high + low (22 bits). A kv head serves at most 8
-// query heads at a time, and the instruction has 16 rows: rows 0-7 hold the high parts, rows 8-15 the low ones, so
-// the exact form costs no instruction more, and both halves of a sum meet in one thread. q is first scaled by a
-// power of two per row (any fp32 size fits fp16); p is relative to its own tile's maximum, so that small weights of
-// other tiles keep their bits, and the tile is joined to the running sums in fp32.
+// (scale s_k) (q . c_j), and a tile of 32 tokens adds s_v sum_j p_j d_j. Both sums run on the codes as they lie in the
+// cache, on the int8 tensor cores (mma.sync m16n8k32): q, scaled by a power of two per row, and the weights p, relative
+// to their own tile's maximum, are 23-bit integers X = x0 + 256 x1 + 65536 x2 with balanced int8 digits, so every digit
+// product is exact in int32 and a result is off only by the rounding of X (2^-22 of the row's largest |q|, 2^-23
+// of the tile's largest weight). A kv head serves at most 8 query heads at a time and the instruction has 16 rows: rows
+// 0-7 hold digit 0 and rows 8-15 digit 1, whose products then meet in one thread; a second instruction holds digit 2.
+// An accumulator starts at the bits of 1.5 * 2^23, so that read as fp32 it is its integer, without a conversion.
+// Each tile is joined to the running maximum and sums in fp32, so weights that are small beside another tile's keep
+// their bits.
 //
-// Bound: HBM bytes of the cache (256 + 8/64 per token and kv head). Per tile and warp the arithmetic is 64 mma, ~350
-// instructions of code conversion and ~100 of softmax, about a third of the issue slots at the memory's rate.
+// Bound: HBM bytes of the cache (256 + 8/64 per token and kv head).
 //
 // Split: all (row, kv head) items lie end to end as tiles, in equal runs over the CTAs and in each CTA over its warps,
-// whatever the lengths are. A warp streams its run through a ring of its own (cp.async, no CTA barrier in the loop).
-// Items that a run cuts are joined in the CTA through shared memory, items that a CTA's run cuts by a second
-// kernel, in the order of the tiles: results do not depend on timing.
+// whatever the lengths are; a border that would cut an item moves to its beginning where that makes no run much longer.
+// A warp streams its run through a ring of its own (cp.async, no CTA barrier in the loop).
+// Items that a run cuts are joined in the CTA through shared memory; items that a CTA's run cuts by the CTA that
+// finishes last, which flags in the workspace tell. Parts are joined in the order of the tiles: results do not
+// depend on timing.
 #include <cuda_runtime.h>
+
+#include <atomic>
+#include <chrono>
 
 #include "kv8_device.cuh"
 
@@ -31,10 +37,11 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;    // tokens
 constexpr int kStages = 3;   // 8 KB each: 128 KB in flight per SM, three times what the latency asks for
 constexpr int kRows = 8;     // query heads of an item
+constexpr int kMinRun = 16;  // tiles of a CTA's run, at least: two for each warp
+constexpr int kSlack = 24;   // tiles by which a run may be longer to keep an item whole (about what a join costs)
 constexpr int kTileBytes = kTile * kHead;       // of K or V
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kPartFloats = kRows * (kHead + 2);  // sums [8][128], maxima [8], weights' sums [8]
-constexpr int kMergeThreads = 256;
 
 // Shared memory: the rings, then a part per warp (an item that began before the warp's run), then the stage notes.
 struct __align__(16) Note {
@@ -50,10 +57,37 @@ constexpr int kScalesOffset = kNotesOffset + kWarps * kStages * (int)sizeof(Note
 constexpr int kSmemBytes = kScalesOffset + kWarps * kStages * 2 * 4;
 static_assert(kSmemBytes + 1024 <= 227 * 1024, "shared memory of one CTA, static part included");
 
-// Workspace: parts [2 * kCtas], then which item each part belongs to. Part 2 c: an item that began before CTA c's
-// run (info = 2 * item + 1 if it ends there, else 2 * item; item = row * subs + sub); part 2 c + 1: one that began in it and goes on. -1: none.
-constexpr size_t kInfoOffset = (size_t)2 * kCtas * kPartFloats * 4;
-constexpr size_t kWorkBytes = kInfoOffset + 2 * kCtas * sizeof(int);
+// Workspace: parts [2 * kCtas], then a flag for each. Part 2 c: an item that began before CTA c's run; part 2 c + 1: one
+// that began in it and goes on. The workspace may hold anything when a call begins, so a flag that is set holds the
+// call's own 64-bit number. A CTA sets its part's flag and then looks at those of all the item's parts; at least the
+// last one finds all of them set. Should two find that, both join the same parts in the same order and write the
+// same bytes. Who joins takes the flags back: a graph's replays use one number, and find no flag set at their start.
+typedef unsigned long long u64;
+constexpr size_t kFlagsOffset = (size_t)2 * kCtas * kPartFloats * 4;
+constexpr size_t kWorkBytes = kFlagsOffset + 2 * kCtas * sizeof(u64);
+
+// One warp: sets flag `mine` of an item's n flags (its first at 0, the others at 1, 3, ...) and tells whether all are set.
+__device__ __forceinline__ bool all_parts(u64* flags, u64 call, int mine, int n) {
+  const int lane = threadIdx.x % 32;
+  if (lane == 0) {
+    __threadfence();  // the part itself first
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(flags + (mine ? 2 * mine - 1 : 0)), "l"(call) : "memory");
+  }
+  __syncwarp();
+  __threadfence();  // sequentially consistent: of two CTAs that set and look, one sees the other's
+  bool all = true;
+  for (int i = lane; i < n; i += 32) {
+    u64 x;
+    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(x) : "l"(flags + (i ? 2 * i - 1 : 0)) : "memory");
+    all = all && x == call;
+  }
+  all = __all_sync(0xffffffffu, all);
+  if (all)
+    for (int i = lane; i < n; i += 32)
+      asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(flags + (i ? 2 * i - 1 : 0)), "l"(0ull) : "memory");
+  __threadfence();
+  return all;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -61,19 +95,21 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+// d = a b + c on int8 codes. `first`: c is the bits of kZero in every place.
+__device__ __forceinline__ void mma(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-// The first product of a sum.
-__device__ __forceinline__ void mma_first(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+constexpr float kZero = 12582912.0f;  // 1.5 * 2^23: kZero + n for |n| < 2^22 has the bits of kZero plus n
+constexpr int kZeroBits = 0x4b400000;
+__device__ __forceinline__ void mma_first(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                          unsigned b1, const int (&zero)[4]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(zero[0]), "r"(zero[1]), "r"(zero[2]), "r"(zero[3]));
 }
 
 // Pairs of fp32 numbers in one instruction.
@@ -103,24 +139,27 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
   return r;
 }
 
-// Two codes to two fp16 numbers: with the sign bit flipped a code is c + 128, as the low byte of 0x64xx it is the
-// number 1024 + 128 + c, and the subtraction is exact. `sel` places bytes 0, 1 (0x5150) or 2, 3 (0x5352).
-template <unsigned kSel>
-__device__ __forceinline__ unsigned codes_to_half2(unsigned flipped) {
-  const unsigned n = __byte_perm(flipped, 0x64646464u, kSel);
-  const unsigned bias = 0x64806480u;
-  const __half2 r = __hsub2(reinterpret_cast<const __half2&>(n), reinterpret_cast<const __half2&>(bias));
-  return reinterpret_cast<const unsigned&>(r);
+// Digits: the bytes of X + 0x808080 are the digits + 128, and flipping their top bits makes them int8. `x` is kZero + X,
+// whose low 24 bits are X + 0x400000.
+__device__ __forceinline__ unsigned digits(float x) { return (__float_as_uint(x) + 0x00408080u) ^ 0x00808080u; }
+// The digits of four numbers, regrouped by digit.
+__device__ __forceinline__ void by_digit(unsigned x0, unsigned x1, unsigned x2, unsigned x3, unsigned (&d)[3]) {
+  const unsigned a = __byte_perm(x0, x1, 0x5140), b = __byte_perm(x2, x3, 0x5140);
+  d[0] = __byte_perm(a, b, 0x5410);
+  d[1] = __byte_perm(a, b, 0x7632);
+  d[2] = __byte_perm(__byte_perm(x0, x1, 0x0062), __byte_perm(x2, x3, 0x0062), 0x5410);
+}
+// Two columns' digit sums to two fp32 numbers: lo is (digit 0, digit 1) of both, hi digit 2, each kZero off. The 256
+// folds digit 0's kZero into digit 1's difference; all steps are exact up to the last two roundings, of 2^-24 each.
+__device__ __forceinline__ u64 join_digits(const int (&lo)[4], const int (&hi)[4]) {
+  const u64 d0 = pair(__int_as_float(lo[0]), __int_as_float(lo[1])), d1 = pair(__int_as_float(lo[2]), __int_as_float(lo[3])),
+            d2 = pair(__int_as_float(hi[0]), __int_as_float(hi[1]));
+  constexpr float kBoth = -(kZero + kZero / 256.0f);
+  const u64 y = fma2(add2(d1, pair(kBoth, kBoth)), pair(256.0f, 256.0f), d0);
+  return fma2(add2(d2, pair(-kZero, -kZero)), pair(65536.0f, 65536.0f), y);
 }
 
-// x, y -> their fp16 roundings and the fp16 roundings of what those leave
-__device__ __forceinline__ void split_half(float x, float y, unsigned& high, unsigned& low) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-  high = reinterpret_cast<const unsigned&>(h);
-  low = reinterpret_cast<const unsigned&>(l);
-}
+__device__ __forceinline__ unsigned word(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
 
 __device__ __forceinline__ void copy16(unsigned dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -137,12 +176,20 @@ __device__ __forceinline__ void copies_wait() {
 // Items of a row: kv heads x chunks of at most 8 query heads.
 struct Layout {
   int group, chunks, subs;
-  __device__ Layout(const Cache& c, const Attend& a)
+  Layout(const Cache& c, const Attend& a)
       : group(a.q_heads / c.heads), chunks((group + kRows - 1) / kRows), subs(c.heads * chunks) {}
   __device__ int head(int sub) const { return sub / chunks; }
   __device__ int first_q(int sub) const { return head(sub) * group + sub % chunks * kRows; }
   __device__ int count(int sub) const { return min(kRows, group - sub % chunks * kRows); }
 };
+
+// x / size for a quotient below 2^20, without the long division.
+__device__ __forceinline__ int run_of(long long x, long long size) {
+  int c = (int)((float)x / (float)size);
+  while (c * size > x) --c;
+  while ((c + 1) * size <= x) ++c;
+  return c;
+}
 
 enum RowKind { kSkip, kEmpty, kWrong, kLive };
 __device__ __forceinline__ RowKind row_kind(const Cache& c, int seq, int len) {
@@ -165,36 +212,47 @@ __device__ __forceinline__ void put_lse(const Attend& a, long long row, int h, f
   if (a.lse) a.lse[row * a.q_heads + h] = m * 0.6931471805599453f + logf(l);
 }
 
-// This lane's dims of one query head, scaled by a power of two and split.
+// This lane's dims of one query head as digits, and what a score of them is multiplied by.
 struct Query {
-  unsigned f[8][4];  // dims 32 q4 + 4 s + {0, 1 | 2, 3} of head g, high and low
+  unsigned d[8][3];  // dims 32 q4 + 4 i + {0 .. 3} of head g
   float scale;       // scale * log2(e) * the power of two that was taken out
 };
 
 template <int kType>
-__global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend a, Layout lay, u64 call) {
   using T = typename TypeOf<kType>::T;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long warp_sum[kWarps];
+  __shared__ long long warp_sum[kWarps], part_from[kWarps], border[2];
+  __shared__ unsigned warp_least[kWarps], warp_most[kWarps];
   __shared__ int4 start[kWarps];  // row, first tile among the row's, length, sequence
-  __shared__ int part_item[2 * kWarps], part_ended[kWarps];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int part_item[2 * kWarps], part_ended[kWarps], is_last;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q4 = lane % 4;
-  const Layout lay(c, a);
 
   // ---- the runs: tiles before each thread's rows, the whole, and where this CTA's warps begin
   const int per_thread = (a.rows + kThreads - 1) / kThreads;
   const int row0 = min(a.rows, (int)threadIdx.x * per_thread), row1 = min(a.rows, row0 + per_thread);
   long long mine = 0;
-  for (int r = row0; r < row1; ++r) mine += row_tiles(c, a, r);
+  unsigned least = ~0u, most = 0;
+  for (int r = row0; r < row1; ++r) {
+    const unsigned n = row_tiles(c, a, r);
+    mine += n;
+    least = min(least, n - 1);  // rows without a tile are not among them
+    most = max(most, n);
+  }
   mine *= lay.subs;
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
   long long upto = mine;
 #pragma unroll
   for (int i = 1; i < 32; i <<= 1) {
     const long long v = __shfl_up_sync(0xffffffffu, upto, i);
     if (lane >= i) upto += v;
   }
-  if (lane == 31) warp_sum[warp] = upto;
+  if (lane == 31) {
+    warp_sum[warp] = upto;
+    warp_least[warp] = least;
+    warp_most[warp] = most;
+  }
   if (threadIdx.x < 2 * kWarps) part_item[threadIdx.x] = -1;
   __syncthreads();
   long long before = upto - mine, all = 0;
@@ -202,19 +260,48 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += warp_sum[w];
     all += warp_sum[w];
+    least = min(least, warp_least[w]);
+    most = max(most, warp_most[w]);
   }
-  const long long per_cta = max((long long)kWarps, (all + kCtas - 1) / kCtas);
-  const long long cta0 = blockIdx.x * per_cta;
-  const int cta_n = (int)max(0ll, min(per_cta, all - cta0));  // the entry point bounds all by 2^40
+  ++least;
+  // Run c begins at tile c * per_cta, or at the beginning of the item there if that stays whole: it is short, or all
+  // are as long and a little longer than a run, so that a run gets one of them or none.
+  const long long per_cta = max((long long)kMinRun, (all + kCtas - 1) / kCtas);
+  const bool alike = least == most && most >= per_cta && most <= per_cta + kSlack;
+  if (threadIdx.x < 2) border[threadIdx.x] = all;
+  __syncthreads();
+  if (mine > 0) {
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      const long long at = (blockIdx.x + i) * per_cta;
+      if (at < before || at >= before + mine) continue;
+      long long pos = before;
+      for (int r = row0; r < row1; ++r) {
+        const int tiles = row_tiles(c, a, r);
+        const long long n = (long long)tiles * lay.subs;
+        if (at < pos + n) {
+          border[i] = tiles <= kSlack || alike ? at - (int)(at - pos) % tiles : at;
+          break;
+        }
+        pos += n;
+      }
+    }
+  }
+  __syncthreads();
+  const long long cta0 = border[0];
+  const int cta_n = (int)(border[1] - cta0);  // the entry point bounds all by 2^40
   const int per_warp = (cta_n + kWarps - 1) / kWarps;
   if (mine > 0 && before < cta0 + cta_n && before + mine > cta0) {
     long long pos = before;
     for (int r = row0; r < row1; ++r) {
       const long long n = (long long)row_tiles(c, a, r) * lay.subs;
+      if (pos + n > cta0 && pos < cta0 + cta_n) {
+        const int4 row = make_int4(r, 0, __ldg(a.row_len + r), __ldg(a.row_seq + r));
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const long long at = cta0 + w * per_warp;
-        if (at >= pos && at < pos + n) start[w] = make_int4(r, (int)(at - pos), __ldg(a.row_len + r), __ldg(a.row_seq + r));
+        for (int w = 0; w < kWarps; ++w) {
+          const long long at = cta0 + w * per_warp;
+          if (at >= pos && at < pos + n) start[w] = make_int4(row.x, (int)(at - pos), row.z, row.w);
+        }
       }
       pos += n;
     }
@@ -295,56 +382,63 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
     };
 
     Query q;
-    auto load_query = [&](int it_row, int it_sub) {
+    auto load_query = [&](int it_row, int it_sub, auto meanwhile) {
       float4 x[8];
-      float top = 0.0f;
+      unsigned top = 0;
       const T* from = static_cast<const T*>(a.q) + it_row * a.q_stride + (long long)(lay.first_q(it_sub) + g) * kHead + q4 * 32;
       const bool live = g < lay.count(it_sub);
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        x[s] = live ? load4(from + s * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[s].x), fabsf(x[s].y)), fmaxf(fabsf(x[s].z), fabsf(x[s].w))));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^-e and 2^e with the row's largest value in [1, 2) after the scaling
-      const int e = top == 0.0f ? 127 : min(253, max(1, (int)(__float_as_uint(top) >> 23)));
-      const float down = __uint_as_float((unsigned)(254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
-      q.scale = a.scale * up * 1.4426950408889634f;
+      for (int i = 0; i < 8; ++i) x[i] = live ? load4(from + i * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      meanwhile();
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        split_half(x[s].x * down, x[s].y * down, q.f[s][0], q.f[s][1]);
-        split_half(x[s].z * down, x[s].w * down, q.f[s][2], q.f[s][3]);
-      }
+      for (int i = 0; i < 8; ++i)
+        top = max(top, max(max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu),
+                           max(__float_as_uint(x[i].z) & 0x7fffffffu, __float_as_uint(x[i].w) & 0x7fffffffu)));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^21 and less of them, with the row's largest value in [2^21, 2^22) after the scaling; a NaN or an infinity in
+      // the row makes all its scores NaN
+      const int e = top == 0 ? 127 : min(253, max(1, (int)(top >> 23)));
+      const float down = __uint_as_float((unsigned)(254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
+      q.scale = top >= 0x7f800000u ? __int_as_float(0x7fc00000) : a.scale * up * (1.4426950408889634f / 2097152.0f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        by_digit(digits(fmaf(x[i].x * down, 2097152.0f, kZero)), digits(fmaf(x[i].y * down, 2097152.0f, kZero)),
+                 digits(fmaf(x[i].z * down, 2097152.0f, kZero)), digits(fmaf(x[i].w * down, 2097152.0f, kZero)), q.d[i]);
     };
 
     int it_row = row, it_sub = sub;
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) load(s);
-    load_query(it_row, it_sub);  // while the first tiles are on their way
+    // the query's loads go first: behind the first tiles' they would wait for 19 MB to come in
+    load_query(it_row, it_sub, [&] {
+#pragma unroll 1
+      for (int s = 0; s < kStages - 1; ++s) load(s);
+    });
 
     float m = -INFINITY, l = 0.0f;  // head g: maximum (base 2) and this lane's share of the sum
     unsigned long long o[16];       // head g: dims 32 q4 + j and 32 q4 + 16 + j
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[j] = 0;
     bool fresh = true, whole = false;
-    int stage = 0;
+    int stage = 0, began = 0;
+    const int zero[4] = {kZeroBits, kZeroBits, kZeroBits, kZeroBits};
     for (int t = 0; t < todo; ++t) {
       copies_wait<kStages - 2>();
-      __syncwarp();
+      __syncwarp();  // all lanes' copies are here, and all lanes are done with the stage before, which is refilled
+      load(stage == 0 ? kStages - 1 : stage - 1);
       const Note note = notes[stage];
       if (fresh) {
         fresh = false;
+        began = t;
         whole = note.flags & kFirst;
-        if (note.row != it_row || note.sub != it_sub) load_query(it_row = note.row, it_sub = note.sub);
+        if (note.row != it_row || note.sub != it_sub) load_query(it_row = note.row, it_sub = note.sub, [] {});
       }
       const uint8_t* kt = ring + stage * kStageBytes;
       const uint8_t* vt = kt + kTileBytes;
       const float ks = note.flags & kBad ? __int_as_float(0x7fc00000) : scales[stage * 2], vs = scales[stage * 2 + 1];
 
       // scores of tokens 8 j + 2 q4 + {0, 1}: the contraction may take the dims in any order, so a lane's 32
-      // codes of token 8 j + g are two 16-byte chunks, four codes for each of the 8 steps
-      float s[4][4];
+      // codes of token 8 j + g are two 16-byte chunks, eight codes for each of the 4 steps
+      int lo[4][4], hi[4][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint4 b[4];
@@ -352,21 +446,29 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
         for (int j = 0; j < 4; ++j)
           b[j] = *reinterpret_cast<const uint4*>(kt + (j * 8 + g) * kHead + (((q4 * 2 + h) ^ g) << 4));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i) {
+          const unsigned(&x)[3] = q.d[h * 4 + i * 2], (&y)[3] = q.d[h * 4 + i * 2 + 1];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const unsigned w = reinterpret_cast<const unsigned*>(&b[j])[i] ^ 0x80808080u;
-            const unsigned b0 = codes_to_half2<0x5150>(w), b1 = codes_to_half2<0x5352>(w);
-            if (h == 0 && i == 0) mma_first(s[j], q.f[0], b0, b1);
-            else mma(s[j], q.f[h * 4 + i], b0, b1);
+            const unsigned b0 = i ? b[j].z : b[j].x, b1 = i ? b[j].w : b[j].y;
+            if (h == 0 && i == 0) {
+              mma_first(lo[j], x[0], x[1], y[0], y[1], b0, b1, zero);
+              mma_first(hi[j], x[2], 0, y[2], 0, b0, b1, zero);
+            } else {
+              mma(lo[j], x[0], x[1], y[0], y[1], b0, b1);
+              mma(hi[j], x[2], 0, y[2], 0, b0, b1);
+            }
           }
+        }
       }
       const float cs = q.scale * ks;
       float p[4][2], tm = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) p[j][i] = (s[j][i] + s[j][i + 2]) * cs;
+      for (int j = 0; j < 4; ++j) {
+        const float2 s = unpair(mul2(join_digits(lo[j], hi[j]), pair(cs, cs)));
+        p[j][0] = s.x;
+        p[j][1] = s.y;
+      }
       if (note.valid < kTile) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -385,18 +487,17 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
         for (int i = 0; i < 2; ++i) p[j][i] = ex2(p[j][i] - tm);
         tl += p[j][0] + p[j][1];
       }
-      const float mn = fmaxf(m, tm), keep = ex2(m - mn), add = ex2(tm - mn), av = add * vs;
+      const float mn = fmaxf(m, tm), keep = ex2(m - mn), add = ex2(tm - mn), av = add * (vs * (1.0f / 4194304.0f));
       m = mn;
       l = l * keep + add * tl;
       const unsigned long long keep2 = pair(keep, keep), av2 = pair(av, av);
 
-      // weights of two 8-token columns are the operand of one 16-token step
-      unsigned pf[2][4];
+      // this lane's weights are what it holds of the operand: 2^22 and less
+      unsigned pd[2][3];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        split_half(p[2 * k][0], p[2 * k][1], pf[k][0], pf[k][1]);
-        split_half(p[2 * k + 1][0], p[2 * k + 1][1], pf[k][2], pf[k][3]);
-      }
+      for (int k = 0; k < 2; ++k)
+        by_digit(digits(fmaf(p[2 * k][0], 4194304.0f, kZero)), digits(fmaf(p[2 * k][1], 4194304.0f, kZero)),
+                 digits(fmaf(p[2 * k + 1][0], 4194304.0f, kZero)), digits(fmaf(p[2 * k + 1][1], 4194304.0f, kZero)), pd[k]);
       uint4 raw[2][4];  // dims 16 g .. 16 g + 15 of tokens 16 k + 2 q4 + {0, 1, 8, 9}
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -407,33 +508,27 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
         }
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        float d[4][4];
+        // 4 x 4 bytes: from four dims of a token to four tokens of a dim
+        unsigned b[2][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          unsigned b[2][4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const unsigned x = reinterpret_cast<const unsigned*>(&raw[k][2 * i])[w];
-            const unsigned y = reinterpret_cast<const unsigned*>(&raw[k][2 * i + 1])[w];
-            const unsigned lo = __byte_perm(x, y, 0x5140) ^ 0x80808080u, hi = __byte_perm(x, y, 0x7362) ^ 0x80808080u;
-            b[i][0] = codes_to_half2<0x5150>(lo);
-            b[i][1] = codes_to_half2<0x5352>(lo);
-            b[i][2] = codes_to_half2<0x5150>(hi);
-            b[i][3] = codes_to_half2<0x5352>(hi);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (k == 0) mma_first(d[i], pf[0], b[0][i], b[1][i]);
-            else mma(d[i], pf[1], b[0][i], b[1][i]);
-          }
+          const unsigned x0 = word(raw[k][0], w), x1 = word(raw[k][1], w), x2 = word(raw[k][2], w), x3 = word(raw[k][3], w);
+          const unsigned l0 = __byte_perm(x0, x1, 0x5140), h0 = __byte_perm(x0, x1, 0x7362);
+          const unsigned l1 = __byte_perm(x2, x3, 0x5140), h1 = __byte_perm(x2, x3, 0x7362);
+          b[k][0] = __byte_perm(l0, l1, 0x5410);
+          b[k][1] = __byte_perm(l0, l1, 0x7632);
+          b[k][2] = __byte_perm(h0, h1, 0x5410);
+          b[k][3] = __byte_perm(h0, h1, 0x7632);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o[w * 4 + i] = fma2(av2, add2(pair(d[i][0], d[i][1]), pair(d[i][2], d[i][3])), mul2(o[w * 4 + i], keep2));
+        for (int i = 0; i < 4; ++i) {
+          int dl[4], dh[4];
+          mma_first(dl, pd[0][0], pd[0][1], pd[1][0], pd[1][1], b[0][i], b[1][i], zero);
+          mma_first(dh, pd[0][2], 0, pd[1][2], 0, b[0][i], b[1][i], zero);
+          o[w * 4 + i] = fma2(av2, join_digits(dl, dh), mul2(o[w * 4 + i], keep2));
+        }
       }
 
-      __syncwarp();  // the stage that is refilled next was read one step ago
-      load(stage == 0 ? kStages - 1 : stage - 1);
       stage = stage + 1 == kStages ? 0 : stage + 1;
 
       const bool ends = note.flags & kLast;
@@ -453,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
             if (q4 == 0) put_lse(a, it_row, h, m, l);
           }
         } else {
-          // an item that goes on: only at the end of the run, when the ring is free to take it
+          // an item that goes on: only at the end of the run, when the ring is free to take it once all lanes have read
           if (whole) {
             copies_wait<0>();
             __syncwarp();
@@ -472,6 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
           if (lane == 0) {
             part_item[2 * warp + whole] = it_row * lay.subs + it_sub;
             if (!whole) part_ended[warp] = ends;
+            else part_from[warp] = cta0 + warp * per_warp + began;
           }
         }
         fresh = true;
@@ -486,7 +582,6 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
   __syncthreads();
 
   // ---- join the warps' parts, warp h head h: part 2 w is warp w's item from before, part 2 w + 1 the one that goes on
-  int* info = reinterpret_cast<int*>(static_cast<uint8_t*>(a.work) + kInfoOffset) + 2 * blockIdx.x;
   const int my_item = lane < 2 * kWarps ? part_item[lane] : -1;
   const float* my_part = lane % 2 ? reinterpret_cast<const float*>(smem + lane / 2 % kWarps * kStages * kStageBytes)
                                   : reinterpret_cast<const float*>(smem + kPartsOffset) + lane / 2 % kWarps * kPartFloats;
@@ -494,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
   const unsigned earlier = live & ((1u << lane) - 1);
   const int prev_item = __shfl_sync(0xffffffffu, my_item, earlier ? 31 - __clz(earlier) : 0);
   unsigned firsts = __ballot_sync(0xffffffffu, my_item >= 0 && !(earlier && prev_item == my_item));
-  int before_info = -1, after_info = -1;
+  int open_item[2] = {-1, -1}, after_warp = 0;  // from before and not done here; going on
   while (firsts) {
     const int first = __ffs(firsts) - 1;
     firsts &= firsts - 1;
@@ -502,8 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
     const int last = 31 - __clz(members), item = __shfl_sync(0xffffffffu, my_item, first);
     const bool ended = last % 2 == 0 && part_ended[last / 2], done = first % 2 == 1 && ended;
     if (!done) {
-      if (first % 2) after_info = item;
-      else before_info = 2 * item + ended;
+      open_item[first % 2] = item;
+      if (first % 2) after_warp = first / 2;
     }
     const int it_row = item / lay.subs, it_sub = item - it_row * lay.subs;
     if (warp >= lay.count(it_sub)) continue;
@@ -517,13 +612,21 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (unsigned rest = members; rest; rest &= rest - 1) {
-      const int p = __ffs(rest) - 1;
-      const float* x = p % 2 ? reinterpret_cast<const float*>(smem + p / 2 * kStages * kStageBytes)
-                             : reinterpret_cast<const float*>(smem + kPartsOffset) + p / 2 * kPartFloats;
-      const float4 v = *reinterpret_cast<const float4*>(x + warp * kHead + lane * 4);
-      const float fp = __shfl_sync(0xffffffffu, f, p);
-      o = make_float4(fmaf(fp, v.x, o.x), fmaf(fp, v.y, o.y), fmaf(fp, v.z, o.z), fmaf(fp, v.w, o.w));
+    for (unsigned rest = members; rest;) {
+      float4 v[kWarps];
+      float fp[kWarps];
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i, rest &= rest - 1) {  // a part too many counts 0 times
+        const int p = rest ? __ffs(rest) - 1 : first;
+        const float* x = p % 2 ? reinterpret_cast<const float*>(smem + p / 2 * kStages * kStageBytes)
+                               : reinterpret_cast<const float*>(smem + kPartsOffset) + p / 2 * kPartFloats;
+        v[i] = *reinterpret_cast<const float4*>(x + warp * kHead + lane * 4);
+        fp[i] = __shfl_sync(0xffffffffu, f, p);
+        if (!rest) v[i] = make_float4(0.f, 0.f, 0.f, 0.f), fp[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i)
+        o = make_float4(fmaf(fp[i], v[i].x, o.x), fmaf(fp[i], v[i].y, o.y), fmaf(fp[i], v[i].z, o.z), fmaf(fp[i], v[i].w, o.w));
     }
     if (done) {
       put_out<T>(a, it_row, lay.first_q(it_sub) + warp, lane * 4, o, 1.0f / l);
@@ -537,9 +640,63 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
       }
     }
   }
-  if (threadIdx.x == 0) {
-    info[0] = before_info;
-    info[1] = after_info;
+
+  // ---- join an item's parts over the CTAs, in the one that finishes last
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int item = open_item[which];
+    if (item < 0) continue;  // the same for all threads
+    const int it_row = item / lay.subs, it_sub = item - it_row * lay.subs;
+    // the item's tiles begin at `from`: in which CTA, and in how many
+    const int tiles = row_tiles(c, a, it_row);
+    const long long from = which ? part_from[after_warp] : cta0 - start[0].y % tiles;
+    const int first_cta = run_of(from, per_cta), n = run_of(from + tiles - 1, per_cta) - first_cta + 1;
+    __syncthreads();
+    if (warp == 0) {
+      // the item's flags: that of part 2 first_cta + 1, then of every second one
+      u64* flags = reinterpret_cast<u64*>(static_cast<uint8_t*>(a.work) + kFlagsOffset) + 2 * first_cta + 1;
+      const bool last = all_parts(flags, call, (int)blockIdx.x - first_cta, n);
+      if (lane == 0) is_last = last;
+    }
+    __syncthreads();
+    if (!is_last || warp >= lay.count(it_sub)) continue;
+    // a factor per part, in the ring's place; a batch of parts is loaded at once, the first beside the maxima
+    const float* parts = static_cast<const float*>(a.work) + (size_t)2 * first_cta * kPartFloats;
+    auto part = [&](int i) { return parts + (size_t)(2 * i + (i == 0)) * kPartFloats; };
+    float* factor = reinterpret_cast<float*>(smem) + warp * kCtas;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAhead = 32;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += kAhead) {
+      float4 v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (i0 + i < n) v[i] = __ldcg(reinterpret_cast<const float4*>(part(i0 + i) + warp * kHead + lane * 4));
+      if (i0 == 0) {
+        for (int i = lane; i < n; i += 32) {
+          factor[i] = __ldcg(part(i) + kRows * kHead + warp);
+          m = fmaxf(m, factor[i]);
+        }
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+        for (int i = lane; i < n; i += 32) {
+          factor[i] = ex2(factor[i] - m);
+          l = fmaf(factor[i], __ldcg(part(i) + kRows * kHead + kRows + warp), l);
+        }
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (i0 + i < n) {
+          const float f = factor[i0 + i];
+          o = make_float4(fmaf(f, v[i].x, o.x), fmaf(f, v[i].y, o.y), fmaf(f, v[i].z, o.z), fmaf(f, v[i].w, o.w));
+        }
+    }
+    put_out<T>(a, it_row, lay.first_q(it_sub) + warp, lane * 4, o, 1.0f / l);
+    if (lane == 0) put_lse(a, it_row, lay.first_q(it_sub) + warp, m, l);
   }
 
   // ---- rows without a tile: nothing cached yet, or an index that is no row of the cache
@@ -556,80 +713,23 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(Cache c, Attend a) {
   }
 }
 
-// Joins the parts of an item that several CTAs' runs share: block (c, h) takes the item that began in CTA c and went
-// on, head h of it. A warp takes every eighth part, its loads independent of one another.
-template <int kType>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(Cache c, Attend a) {
-  using T = typename TypeOf<kType>::T;
-  constexpr int kMergeWarps = kMergeThreads / 32;
-  __shared__ float4 sum[kMergeWarps][32];
-  __shared__ float top[kMergeWarps], total[kMergeWarps], factor[kCtas];
-  static_assert(kCtas <= kMergeThreads, "a thread per part");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const float* work = static_cast<const float*>(a.work);
-  const int* info = reinterpret_cast<const int*>(static_cast<const uint8_t*>(a.work) + kInfoOffset);
-  const int cta = blockIdx.x, h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int item = info[2 * cta + 1];
-  if (item < 0) return;
-  const Layout lay(c, a);
-  const int it_row = item / lay.subs, it_sub = item - it_row * lay.subs;
-  if (h >= lay.count(it_sub)) return;
-  // part 0 is 2 cta + 1, part i the first one of CTA cta + i, up to the CTA where the item ends
-  const int i = threadIdx.x, x = i > 0 && cta + i < kCtas ? info[2 * (cta + i)] : -1;
-  const bool mine = i == 0 || x >> 1 == item;
-  const float* my_part = work + (size_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * kPartFloats;
-  const float pm = mine ? my_part[kRows * kHead + h] : -INFINITY, pl = mine ? my_part[kRows * kHead + kRows + h] : 0.0f;
-  float m = pm;
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  if (lane == 0) top[warp] = m;
-  const int n = __syncthreads_count(mine);
-#pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, top[w]);
-  const float f = mine ? ex2(pm - m) : 0.0f;
-  if (i < kCtas) factor[i] = f;
-  float l = mine ? f * pl : 0.0f;
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
-  if (lane == 0) total[warp] = l;
-  __syncthreads();
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 10
-  for (int p = warp; p < n; p += kMergeWarps) {
-    const float4 v = *reinterpret_cast<const float4*>(work + (size_t)(2 * (cta + p) + (p == 0)) * kPartFloats + h * kHead + lane * 4);
-    const float fp = factor[p];
-    o = make_float4(fmaf(fp, v.x, o.x), fmaf(fp, v.y, o.y), fmaf(fp, v.z, o.z), fmaf(fp, v.w, o.w));
-  }
-  sum[warp][lane] = o;
-  __syncthreads();
-  if (warp != 0) return;
-  l = total[0];
-#pragma unroll
-  for (int w = 1; w < kMergeWarps; ++w) {
-    const float4 v = sum[w][lane];
-    l += total[w];
-    o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-  }
-  put_out<T>(a, it_row, lay.first_q(it_sub) + h, lane * 4, o, 1.0f / l);
-  if (lane == 0) put_lse(a, it_row, lay.first_q(it_sub) + h, m, l);
+// A number that no earlier call had, in the upper 48 bits.
+u64 call_number() {
+  static std::atomic<u64> next{(u64)std::chrono::steady_clock::now().time_since_epoch().count()};
+  u64 x = next.fetch_add(0x9e3779b97f4a7c15ull);
+  x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;
+  x = (x ^ (x >> 27)) * 0x94d049bb133111ebull;
+  x = (x ^ (x >> 31)) & ~0xffffull;
+  return x ? x : 1ull << 16;
 }
 
 template <int kType>
 cudaError_t launch(const Cache& c, const Attend& a, cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(split_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  const cudaError_t e =
+      cudaFuncSetAttribute(attention_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return e;
-  split_kernel<kType><<<kCtas, kThreads, kSmemBytes, s>>>(c, a);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kCtas, kRows);
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<kType>, c, a);
+  attention_kernel<kType><<<kCtas, kThreads, kSmemBytes, s>>>(c, a, Layout(c, a), call_number());
+  return cudaGetLastError();
 }
 
 }  // namespace
