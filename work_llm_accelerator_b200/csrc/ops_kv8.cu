@@ -67,6 +67,7 @@ bool cache_ok(const char* op, const qwen_b200_kv8_cache* c) {
     return false;
   }
   return range_ok(op, "n_blocks", c->n_blocks, 1, INT32_MAX) && range_ok(op, "n_kv_heads", c->n_kv_heads, 1, 1024) &&
+         range_ok(op, "n_blocks * n_kv_heads", (long long)c->n_blocks * c->n_kv_heads, 1, INT32_MAX) &&
          range_ok(op, "n_seqs", c->n_seqs, 1, INT32_MAX) &&
          range_ok(op, "max_blocks", c->max_blocks, 1, INT32_MAX / kv8::kBlock);
 }
