@@ -252,3 +252,48 @@ def test_many_rows_repeat_exactly_and_without_probs():
     b, q = run(x, us, top_p=[0.9] * 400)
     c, none = run(x, us, top_p=[0.9] * 400, probs=False)
     assert (a == b).all() and (p == q).all() and (a == c).all() and (none == -9).all()
+
+
+def test_engine_samples_from_its_own_logits():
+    """A generation loop: prompt, then batched steps whose tokens are sampled on the device from the engine's logits."""
+    from work_llm_accelerator_b200 import host
+
+    eng = host.Engine(0, 8, max_seqs=3, max_len=256)
+    try:
+        eng.init_synthetic(5)
+        with pytest.raises(host.EngineError):
+            eng.sample([0.5])  # no call yet
+        eng.set_option("logits", 1)
+        r = np.random.RandomState(0)
+        nxt = []
+        for slot in range(3):
+            greedy = eng.prefill(slot, r.randint(0, host.VOCAB, 5 + slot))
+            x = eng.read_logits(1)[0]
+            tokens, probs = eng.sample([0.7], temperature=[0.0])
+            assert tokens[0] == greedy == int(x.argmax()) and probs[0] == 1.0
+            nxt.append(int(tokens[0]))
+        for step in range(4):
+            eng.decode([0, 1, 2], nxt)
+            x = eng.read_logits(3)
+            kw = dict(temperature=[0.7, 1.0, 1.2], top_k=[50, 0, 7], min_p=[0.0, 0.01, 0.0])
+            us, want = [], []
+            for i in range(3):
+                f = {k: (float(np.float32(v[i])) if k != "top_k" else v[i]) for k, v in kw.items()}
+                ids, w = km.kept(x[i], **f)
+                u, at = middle(w, r)
+                us.append(u)
+                want.append((int(ids[at]), w[at] / w.sum()))
+            tokens, probs = eng.sample(us, **kw)
+            assert [int(t) for t in tokens] == [t for t, _ in want]
+            np.testing.assert_allclose(probs, [p for _, p in want], rtol=2.0**-18)
+            nxt = [int(t) for t in tokens]
+        with pytest.raises(host.EngineError):
+            eng.sample([0.5, 0.5])  # the last call had three rows
+        with pytest.raises(ValueError):
+            eng.sample([0.5] * 3, top_k=[1, 2])
+        eng.set_option("logits", 0)
+        eng.decode([0, 1, 2], nxt)
+        with pytest.raises(host.EngineError):
+            eng.sample([0.5] * 3)  # kept no logits
+    finally:
+        eng.close()

@@ -29,6 +29,7 @@
 #include "tgemm.h"
 #include "qwen_kernels.cuh"
 #include "runtime.h"
+#include "sample.h"
 
 #include "exact.h"
 
@@ -190,6 +191,9 @@ struct qwen_engine {
   float* dump = nullptr;
   float* logits = nullptr;
   int last_rows = 0;
+  int logits_rows = 0;           // rows of `logits` that the last call wrote, 0 if it kept none
+  float* sample_io = nullptr;    // settings and results of qwen_engine_sample, 7 words a row
+  int sample_cap = 0;
   // rope tables
   float *rope_dec_cos = nullptr, *rope_dec_sin = nullptr, *rope_pre_cos = nullptr, *rope_pre_sin = nullptr;
   int rope_dec_len = 0, rope_pre_len = 0;
@@ -996,6 +1000,7 @@ void qwen_engine_destroy(qwen_engine* e) {
                   e->bs1_buf.h, e->bs1_buf.hmax, e->bs1_buf.steps, e->bs1_sync, e->d_item_off1, e->d_items1};
   for (void* p : ptrs) cudaFree(p);
   cudaFree(e->trace);
+  cudaFree(e->sample_io);
   cudaFree(e->lm.planes);
   cudaFree(e->p_planes);
   cudaFree(e->p_steps);
@@ -1134,6 +1139,11 @@ int qwen_engine_set_option(qwen_engine* e, const char* name, long long value) {
 
 namespace {
 
+void note_rows(qwen_engine* e, int n) {
+  e->last_rows = n;
+  e->logits_rows = e->keep_logits || e->exact ? n : 0;
+}
+
 // n prompt tokens into `slot` after the `past` tokens it holds (0: a fresh prompt).
 int prefill_at(qwen_engine* e, int slot, const int32_t* tokens, int n, int past, int32_t* next_token) {
   if (n <= 0 || past < 0 || past + n > e->max_len) {
@@ -1155,7 +1165,7 @@ int prefill_at(qwen_engine* e, int slot, const int32_t* tokens, int n, int past,
   E_TRY(cudaMemcpyAsync(e->h_io + 12, e->d_next, 4, cudaMemcpyDeviceToHost, s));
   E_TRY(cudaStreamSynchronize(s));
   e->seq_len[slot] = past + n;
-  e->last_rows = 1;
+  note_rows(e, 1);
   e->dev_slots.clear();
   if (next_token) *next_token = e->h_io[12];
   return 0;
@@ -1208,7 +1218,7 @@ int qwen_engine_decode(qwen_engine* e, const int32_t* slots, const int32_t* toke
       next_tokens[i] = e->hb_io[3 * e->batch_cap + i];
       e->seq_len[slots[i]] += 1;
     }
-    e->last_rows = n;
+    note_rows(e, n);
     return 0;
   }
   for (int base = 0; base < n; base += kGemvMaxTokens) {
@@ -1238,7 +1248,7 @@ int qwen_engine_decode(qwen_engine* e, const int32_t* slots, const int32_t* toke
       next_tokens[base + i] = e->h_io[12 + i];
       e->seq_len[slots[base + i]] += 1;
     }
-    e->last_rows = nt;
+    note_rows(e, nt);
   }
   return 0;
 }
@@ -1248,6 +1258,7 @@ int qwen_engine_bench_decode(qwen_engine* e, const int32_t* slots, const int32_t
   if (!e || !slots || !first_tokens || n <= 0 || steps <= 0 || warmup < 0) return kStatusInvalid;
   if (n > kGemvMaxTokens && !batched_ok(e, n)) return kStatusInvalid;
   E_TRY(cudaSetDevice(e->device));
+  e->logits_rows = 0;
   if (n > kGemvMaxTokens) {
     int max_end = 0;
     for (int i = 0; i < n; ++i) {
@@ -1516,6 +1527,40 @@ int qwen_engine_read_logits(qwen_engine* e, float* out, long long n_floats) {
   return 0;
 }
 
+int qwen_engine_sample(qwen_engine* e, int n, const float* temperature, const int32_t* top_k, const float* top_p,
+                       const float* min_p, const float* uniforms, int32_t* tokens, float* probs) {
+  if (!e || !uniforms || !tokens || n <= 0) return kStatusInvalid;
+  if (n != e->logits_rows) {
+    set_error("qwen_engine_sample: %d rows, but the last call kept the logits of %d (option \"logits\")", n, e->logits_rows);
+    return kStatusInvalid;
+  }
+  E_TRY(cudaSetDevice(e->device));
+  if (e->sample_cap < n) {
+    E_TRY(cudaStreamSynchronize(e->stream));
+    cudaFree(e->sample_io);
+    e->sample_io = nullptr;
+    e->sample_cap = 0;
+    E_TRY(dalloc(&e->sample_io, (size_t)7 * n));
+    e->sample_cap = n;
+  }
+  // one row of the buffer per setting, one copy each way
+  std::vector<float> io((size_t)5 * n);
+  const void* from[5] = {uniforms, temperature, top_k, top_p, min_p};
+  for (int i = 0; i < 5; ++i)
+    if (from[i]) memcpy(io.data() + (size_t)i * n, from[i], (size_t)n * 4);
+  float* d = e->sample_io;
+  E_TRY(cudaMemcpyAsync(d, io.data(), io.size() * 4, cudaMemcpyHostToDevice, e->stream));
+  const sampling::Sample a{e->logits, n, kVocab, kVocab, temperature ? d + n : nullptr,
+                           top_k ? reinterpret_cast<int*>(d + 2 * n) : nullptr, top_p ? d + 3 * n : nullptr,
+                           min_p ? d + 4 * n : nullptr, d, reinterpret_cast<int*>(d + 5 * n), d + 6 * n};
+  E_TRY(sampling::launch_sample(a, 0, e->stream));
+  E_TRY(cudaMemcpyAsync(io.data(), d + 5 * n, (size_t)2 * n * 4, cudaMemcpyDeviceToHost, e->stream));
+  E_TRY(cudaStreamSynchronize(e->stream));
+  memcpy(tokens, io.data(), (size_t)n * 4);
+  if (probs) memcpy(probs, io.data() + n, (size_t)n * 4);
+  return 0;
+}
+
 int qwen_engine_decode_device(qwen_engine* e, const int32_t* slots, const int32_t* d_tokens, int n,
                               int32_t* d_next) {
   if (!e || !slots || !d_tokens || !d_next || n <= 0) return kStatusInvalid;
@@ -1561,7 +1606,7 @@ int qwen_engine_decode_device(qwen_engine* e, const int32_t* slots, const int32_
   advance_pos_kernel<<<(n + 255) / 256, 256, 0, e->stream>>>(e->d_pos, n);
   E_TRY(cudaGetLastError());
   for (int i = 0; i < n; ++i) e->seq_len[slots[i]] += 1;
-  e->last_rows = n;
+  note_rows(e, n);
   return 0;
 }
 

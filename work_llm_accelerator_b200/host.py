@@ -203,6 +203,7 @@ def _configure_engine(lib: ctypes.CDLL) -> None:
     lib.qwen_engine_set_option.argtypes = [vp, ctypes.c_char_p, ctypes.c_longlong]
     lib.qwen_engine_read_hidden.argtypes = [vp, _F, ctypes.c_longlong]
     lib.qwen_engine_read_logits.argtypes = [vp, _F, ctypes.c_longlong]
+    lib.qwen_engine_sample.argtypes = [vp, i, vp, vp, vp, vp, _F, _I32, vp]
     lib.qwen_engine_read_trace.argtypes = [vp, np.ctypeslib.ndpointer(np.uint64, flags="C_CONTIGUOUS"),
                                            ctypes.c_longlong, ctypes.POINTER(ctypes.c_int),
                                            ctypes.POINTER(ctypes.c_int)]
@@ -228,7 +229,7 @@ def _configure_engine(lib: ctypes.CDLL) -> None:
               "qwen_engine_profile_kernels", "qwen_engine_read_trace", "qwen_engine_profile_decode",
               "qwen_engine_profile_batched", "qwen_engine_nccl_unique_id", "qwen_engine_nccl_init",
               "qwen_engine_gather_tokens", "qwen_engine_gather_tokens_async", "qwen_engine_gather_join",
-              "qwen_engine_read_kv_hf", "qwen_engine_write_kv_hf",
+              "qwen_engine_read_kv_hf", "qwen_engine_write_kv_hf", "qwen_engine_sample",
               "qwen_engine_prefill_chunk"):
         getattr(lib, n).restype = i
 
@@ -354,6 +355,21 @@ class Engine:
         out = np.zeros(rows * VOCAB, np.float32)
         _check(self.lib.qwen_engine_read_logits(self.handle, out, out.size), "read_logits")
         return out.reshape(rows, VOCAB)
+
+    def sample(self, uniforms: Sequence[float], temperature: Sequence[float] | None = None,
+               top_k: Sequence[int] | None = None, top_p: Sequence[float] | None = None,
+               min_p: Sequence[float] | None = None) -> tuple[np.ndarray, np.ndarray]:
+        """(tokens, probabilities) sampled from the last call's logits, a row per uniform number (option "logits" on;
+        include/qwen_b200_engine.h). Settings are per row, None: off."""
+        u = np.ascontiguousarray(uniforms, np.float32)
+        rows = [None if v is None else np.ascontiguousarray(v, t)
+                for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        if any(v is not None and v.shape != u.shape for v in rows) or u.ndim != 1:
+            raise ValueError("sample: one setting per uniform number")
+        tokens, probs = np.zeros(u.size, np.int32), np.zeros(u.size, np.float32)
+        _check(self.lib.qwen_engine_sample(self.handle, u.size, *(None if v is None else v.ctypes.data for v in rows), u,
+                                           tokens, probs.ctypes.data), "sample")
+        return tokens, probs
 
     def bench_decode(self, slots: Sequence[int], first_tokens: Sequence[int], steps: int, warmup: int) -> float:
         s = np.ascontiguousarray(slots, np.int32)
