@@ -35,7 +35,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBuckets = 2048;
 constexpr int kPerThread = kBuckets / kThreads;
-constexpr int kList = 1024;  // tokens that are sorted at once
+constexpr int kList = 2048;  // tokens that are sorted at once
 constexpr int kOrderBits = 50;
 constexpr int kDigit = 11;        // bits by which a crowded bucket is narrowed at a time
 constexpr int kFold = 1 << 15;    // logits whose q, below 2^17 each, fit a 32-bit sum
@@ -178,11 +178,31 @@ struct Scale {
 
 // What the leader asks of every CTA.
 enum Op { kDone, kGather, kHistogram, kCountLeast };
+constexpr int kRanges = 4;
 struct Command {
   int op, first, last;  // buckets
   int bits;             // of the order that are fixed
   u64 prefix;           // their value
+  // kGather, with more than one range: of first .. last only the buckets in these (closed)
+  int ranges, from[kRanges], to[kRanges];
 };
+
+// The first of places 0 .. n - 1 that satisfies a condition which stays true from there on, n - 1 if none does: 32 places
+// at a time. Every warp that takes part finds the same.
+template <typename F>
+__device__ __forceinline__ int first_of(int n, F holds) {
+  const int lane = threadIdx.x % 32;
+  int from = 0, left = n;
+  while (left > 1) {
+    const int step = (left + 31) / 32, end = min((lane + 1) * step, left);  // this lane's last place, from 1
+    const unsigned hit = __ballot_sync(0xffffffffu, holds(from + end - 1));
+    const int first = hit ? __ffs(hit) - 1 : 31;
+    const int next = min(first * step, left - 1);
+    left = min(step, left - next);
+    from += next;
+  }
+  return from;
+}
 
 struct Sums {
   unsigned count[kBuckets];
@@ -194,22 +214,11 @@ struct Running {
   double mass[kBuckets];
   // the first bucket at which the count or the mass suffices (one with tokens in it), the last one if none does
   __device__ int find_count(unsigned k) const {
-    int lo = 0, hi = kBuckets - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (count[mid] >= k) hi = mid;
-      else lo = mid + 1;
-    }
-    return lo;
+    return first_of(kBuckets, [&](int b) { return count[b] >= k; });
   }
   __device__ int find_mass(double want, bool more) const {
-    int lo = 0, hi = kBuckets;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (more ? mass[mid] > want : mass[mid] >= want) hi = mid;
-      else lo = mid + 1;
-    }
-    return lo < kBuckets ? lo : find_count(count[kBuckets - 1]);
+    const int b = first_of(kBuckets, [&](int i) { return more ? mass[i] > want : mass[i] >= want; });
+    return b < kBuckets - 1 ? b : find_count(count[kBuckets - 1]);
   }
   __device__ unsigned before(int b) const { return b ? count[b - 1] : 0; }
   __device__ double mass_before(int b) const { return b ? mass[b - 1] : 0.0; }
@@ -224,9 +233,11 @@ struct Shared {
     };
   };
   Sums sums;       // this CTA's
-  Sums total;      // the leader's: of all CTAs
+  union {
+    Sums total;    // the leader's: of all CTAs
+    Running bins;  // then over the bins of a crowded bucket, best first
+  };
   Running row;     // the leader's: over the buckets
-  Running bins;    // the leader's: of the bins of a crowded bucket, best first
   u64 best[kMaxCluster];
   Command command;
   int listed, counted;
@@ -373,35 +384,70 @@ struct Row {
       sh.sums.q[first + i] = q[i];
     }
   }
-  __device__ void gather(const Command& cmd) {
-    int* listed = at_rank(&sh.listed, 0);
-    u64* to = at_rank(sh.list, 0);
-    const int shift = kOrderBits - cmd.bits;
-    // An interval that holds the logits of those buckets, a little wider: two comparisons settle almost every logit.
-    const float a = scale.top - (float)(cmd.last + 1) / scale.c, b = scale.top - (float)cmd.first / scale.c;
-    const float wide = (fabsf(scale.top) + fmaxf(fabsf(a), fabsf(b))) * 1e-6f;
-    const float v_low = a - wide, v_high = b + wide;  // NaN or infinite: every logit is looked at
-    for_each<kLight>(0, n, [&](const auto& e, int at) {
-      constexpr int kN = (int)(sizeof(e) / sizeof(float));
-      bool any = top_infinite;
+  // Appends the tokens of the command's buckets to the leader's list. kMany: of several ranges of buckets.
+  template <bool kMany>
+  __device__ __forceinline__ void gather() {
+    const Command& cmd = sh.command;
+    int* const listed = at_rank(&sh.listed, 0);
+    u64* const to = at_rank(sh.list, 0);
+    const int shift = kOrderBits - cmd.bits, first_index = lo;
+    const bool narrowed = cmd.bits > 0, infinite = top_infinite;
+    const u64 prefix = cmd.prefix;
+    const Scale sc = scale;
+    auto append = [&](float v, int i) {
+      const u64 o = order_of(v + 0.0f, first_index + i);
+      if (narrowed && o >> shift != prefix) return;
+      const int place = atomicAdd(listed, 1);
+      if (place < kList) to[place] = o;
+    };
+    if (kMany) {
+      float from[kRanges], end[kRanges];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) any = any || !(e[i] < v_low || e[i] > v_high);
-      if (!any) return;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const float v = seen(e[i]), t = scale.steps(v);
-        if (!(t >= (float)cmd.first && t < (float)(cmd.last + 1))) continue;
-        const u64 o = order_of(v + 0.0f, lo + at + i);
-        if (cmd.bits && o >> shift != cmd.prefix) continue;
-        const int place = atomicAdd(listed, 1);
-        if (place < kList) to[place] = o;
+      for (int k = 0; k < kRanges; ++k) {
+        from[k] = k < cmd.ranges ? (float)cmd.from[k] : 1.0f;
+        end[k] = k < cmd.ranges ? (float)(cmd.to[k] + 1) : 0.0f;
       }
-    });
+      for_each<kLight / 2>(0, n, [&](const auto& e, int at) {
+        constexpr int kN = (int)(sizeof(e) / sizeof(float));
+        unsigned in = 0;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const float t = sc.steps(infinite ? seen(e[i]) : e[i]);
+          bool one = false;
+#pragma unroll
+          for (int k = 0; k < kRanges; ++k) one = one || (t >= from[k] && t < end[k]);
+          in |= one ? 1u << i : 0u;
+        }
+        if (in == 0) return;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+          if (in >> i & 1) append(seen(e[i]), at + i);
+      });
+    } else {
+      // An interval that holds the logits of the buckets, a little wider: two comparisons settle almost every logit.
+      const float from = (float)cmd.first, end = (float)(cmd.last + 1);
+      const float a = sc.top - end / sc.c, b = sc.top - from / sc.c;
+      const float wide = (fabsf(sc.top) + fmaxf(fabsf(a), fabsf(b))) * 1e-6f;
+      const float v_low = a - wide, v_high = b + wide;  // NaN or infinite: every logit is looked at
+      for_each<kLight>(0, n, [&](const auto& e, int at) {
+        constexpr int kN = (int)(sizeof(e) / sizeof(float));
+        bool any = infinite;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) any = any || !(e[i] < v_low || e[i] > v_high);
+        if (!any) return;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const float v = seen(e[i]), t = sc.steps(v);
+          if (t >= from && t < end) append(v, at + i);
+        }
+      });
+    }
   }
   __device__ bool reaches_least(float v) const {
     return exp(((double)v - (double)scale.top) / (double)temperature) >= (double)least || v == scale.top;
   }
-  __device__ void count_least(const Command& cmd) {
+  __device__ __forceinline__ void count_least() {
+    const Command& cmd = sh.command;
     int* counted = at_rank(&sh.counted, 0);
     for_each<1>(0, n, [&](const auto& e, int) {
 #pragma unroll
@@ -411,10 +457,15 @@ struct Row {
       }
     });
   }
-  __device__ void serve(const Command& cmd) {
-    if (cmd.op == kGather) gather(cmd);
-    else if (cmd.op == kCountLeast) count_least(cmd);
-    else if (cmd.op == kHistogram) {
+  // What the command asks for; not inlined, so that its loops have the registers to themselves.
+  __device__ __noinline__ void serve() {
+    const Command& cmd = sh.command;
+    if (cmd.op == kGather) {
+      if (cmd.ranges > 1) gather<true>();
+      else gather<false>();
+    } else if (cmd.op == kCountLeast) {
+      count_least();
+    } else if (cmd.op == kHistogram) {
       add_up<true>(cmd);
       share_sums();
     }
@@ -427,7 +478,7 @@ struct Row {
     if (threadIdx.x < kCl) *at_rank(&sh.command, threadIdx.x) = cmd;
     sync_all();
     if (cmd.op == kDone) return;
-    serve(cmd);
+    serve();
     sync_all();
   }
 
@@ -511,6 +562,7 @@ struct Row {
         wc += sh.warp_count[w];
         wm += sh.warp_mass[w];
       }
+    // every thread has read its sums by now: `to` may lie over them
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       to.count[first + i] = wc + sc + c[i];
@@ -525,13 +577,12 @@ struct Row {
     int size = 2;
     while (size < n_list) size <<= 1;
     for (int i = n_list + threadIdx.x; i < size; i += kThreads) list[i] = 0;
-    // steps within 64 neighbours need only their own warp, which holds them
+    // a warp's turn covers 64 neighbours: steps within them need only their own warp
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
-        if (j >= 32 || (j == k >> 1)) __syncthreads();
+        if (j >= 32 || j == k >> 1) __syncthreads();
         else __syncwarp();
-        const int t = threadIdx.x;
-        if (t < size / 2) {
+        for (int t = threadIdx.x; t < size / 2; t += kThreads) {
           const int i = 2 * t - (t & (j - 1)), p = i + j;
           const u64 u = list[i], v = list[p];
           if ((u < v) == ((i & k) == 0)) {
@@ -541,10 +592,15 @@ struct Row {
         }
       }
     __syncthreads();
-    const int i0 = 2 * threadIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const double w0 = i0 < n_list ? scale.weight(value_of(list[i0])) : 0.0;
-    const double w1 = i0 + 1 < n_list ? scale.weight(value_of(list[i0 + 1])) : 0.0;
-    double s = w0 + w1;
+    constexpr int kEach = kList / kThreads;
+    const int each = (n_list + kThreads - 1) / kThreads, i0 = each * threadIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    double w[kEach], own = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (i < each && i0 + i < n_list) own += scale.weight(value_of(list[i0 + i]));
+      w[i] = own;
+    }
+    double s = own;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
       const double v = __shfl_up_sync(0xffffffffu, s, i);
@@ -554,29 +610,33 @@ struct Row {
     s = __shfl_up_sync(0xffffffffu, s, 1);
     if (lane == 0) s = 0.0;
     __syncthreads();
+    double before = 0.0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-      if (w < warp) s += sh.warp_mass[w];
-    sh.prefix[i0] = s + w0;
-    sh.prefix[i0 + 1] = s + (w0 + w1);
+    for (int i = 0; i < kWarps; ++i)
+      if (i < warp) before += sh.warp_mass[i];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (i < each && i0 + i < n_list) sh.prefix[i0 + i] = before + (s + w[i]);
     __syncthreads();
   }
-  // The first place of the sorted list that satisfies reached(place); the last one if none does.
-  template <typename F>
-  __device__ int first_place(int n_list, F reached) const {
-    int a = 0, b = n_list - 1;
-    while (a < b) {
-      const int mid = (a + b) / 2;
-      if (reached(mid)) b = mid;
-      else a = mid + 1;
-    }
-    return a;
-  }
-
+  // A mass inside bucket b, kept from leaving it by the rounding of its sum.
+  __device__ double within(int b, double m) const { return fmin(fmax(m, sh.row.mass_before(b)), sh.row.mass[b]); }
   // Inside bucket b: the cut at the first token with at least `need` tokens of the bucket up to it (need > 0), or a mass
-  // of everything up to it that reaches (more: exceeds) want; at most `most` tokens. Also that token.
-  __device__ Cut resolve(int b, unsigned need, double want, bool more, unsigned most, u64& order) {
-    Command cmd{kGather, b, b, 0, 0};
+  // of everything up to it that reaches (more: exceeds) want; at most `most` tokens. Also that token. `listed`: the
+  // sorted list holds all of the bucket, among others.
+  __device__ Cut resolve(int b, unsigned need, double want, bool more, unsigned most, int listed, u64& order) {
+    if (listed) {
+      const int from = first_of(listed, [&](int i) { return scale.bucket(value_of(sh.list[i])) >= b; });
+      const unsigned n_in = sh.row.count[b] - sh.row.before(b);
+      const double m0 = sh.row.mass_before(b) - (from ? sh.prefix[from - 1] : 0.0);
+      const int at = first_of((int)min(min(most, n_in), (unsigned)(listed - from)), [&](int i) {
+        const double m = m0 + sh.prefix[from + i];
+        return need ? (unsigned)i + 1 >= need : (more ? m > want : m >= want);
+      });
+      order = sh.list[from + at];
+      return {b, (unsigned)at + 1, within(b, m0 + sh.prefix[from + at])};
+    }
+    Command cmd{kGather, b, b, 0, 0, 0, {}, {}};
     unsigned c0 = 0, n_in = sh.row.count[b] - sh.row.before(b);
     double m0 = sh.row.mass_before(b);
     most = min(most, n_in);
@@ -596,11 +656,11 @@ struct Row {
     }
     ask(cmd);
     sort_list((int)n_in);
-    const int at = first_place(min(n_in, most - c0), [&](int i) {
+    const int at = first_of(min(n_in, most - c0), [&](int i) {
       return need ? c0 + i + 1 >= need : (more ? m0 + sh.prefix[i] > want : m0 + sh.prefix[i] >= want);
     });
     order = sh.list[at];
-    return {b, c0 + at + 1, m0 + sh.prefix[at]};
+    return {b, c0 + at + 1, within(b, m0 + sh.prefix[at])};
   }
 
   __device__ void lead(float u, int k, float p, u64 best, u64& order, double& total) {
@@ -623,63 +683,87 @@ struct Row {
     }
     const double draw = u > 0.0f ? (double)u : 0.0;
 
-    // a bucket that no kept token lies behind, and that the sums which decide do not reach behind: top_p after top_k
-    // needs the sum of all that top_k keeps
-    if (k || use_p || use_least) {
-      int bound = kBuckets - 1;
-      if (k) bound = row.find_count(k);
-      else if (use_p) bound = row.find_mass((double)p * row.mass[kBuckets - 1], false);
-      if (use_least && !(k && use_p)) bound = min(bound, least_bucket);
-      const int n_in = (int)row.count[bound];
-      if (n_in <= kList) {  // few: sort them all and filter there
-        ask({kGather, 0, bound, 0, 0});
-        sort_list(n_in);
-        int kept = k ? min(k, n_in) : n_in;
-        if (use_p) {
-          // without top_k the whole sum counts, behind the bound too
-          const double want = (double)p * (k ? sh.prefix[kept - 1] : row.mass[kBuckets - 1]);
-          kept = 1 + first_place(kept, [&](int i) { return sh.prefix[i] >= want; });
-        }
-        if (use_least) {
-          const int out = first_place(kept, [&](int i) { return !reaches_least(value_of(sh.list[i])); });
-          if (!reaches_least(value_of(sh.list[out]))) kept = max(1, out);
-        }
-        total = sh.prefix[kept - 1];
-        const double want = draw * total;
-        order = sh.list[first_place(kept, [&](int i) { return sh.prefix[i] > want; })];
-        return;
-      }
+    // The buckets that borders and draw may fall in, from the sums alone: a border inside a bucket leaves the mass up to
+    // it between that before and that behind the bucket, and so what depends on it between two buckets. Mostly they
+    // hold few tokens, which are gathered and sorted at once.
+    const double whole = row.mass[kBuckets - 1];
+    Command cmd{kGather, kBuckets, 0, 0, 0, 0, {}, {}};
+    unsigned listed = 0;
+    auto want_range = [&](int from, int to) {
+      cmd.from[cmd.ranges] = from;
+      cmd.to[cmd.ranges++] = to;
+      cmd.first = min(cmd.first, from);
+      cmd.last = max(cmd.last, to);
+      listed += row.count[to] - row.before(from);
+    };
+    double low = whole, high = whole;  // of the mass that is kept
+    int cut_to = kBuckets - 1;         // no kept token lies behind
+    if (k) {
+      cut_to = row.find_count(k);
+      low = row.mass_before(cut_to);
+      high = row.mass[cut_to];
+      if (row.count[cut_to] == (unsigned)k) low = high;
+      else want_range(cut_to, cut_to);
+    }
+    if (use_p) {
+      const int from = row.find_mass((double)p * low, false), to = min(cut_to, row.find_mass((double)p * high, false));
+      want_range(from, to);
+      low = row.mass_before(from);
+      high = row.mass[to];
+      cut_to = to;
+    }
+    if (use_least && least_bucket <= cut_to) {
+      if (row.count[least_bucket] > row.before(least_bucket)) want_range(least_bucket, least_bucket);
+      low = min(low, row.mass_before(least_bucket));
+      high = row.mass[least_bucket];
+    }
+    want_range(row.find_mass(draw * low, true), min(cut_to, row.find_mass(draw * high, true)));
+    int n_list = 0;
+    if (listed <= kList) {
+      ask(cmd);
+      n_list = sh.listed;
+      sort_list(n_list);
     }
 
     Cut cut{kBuckets, 0, row.mass[kBuckets - 1]};  // nothing is cut off
     if (k) {
       const int b = row.find_count(k);
       if (row.count[b] == (unsigned)k) cut = {b, (unsigned)k - row.before(b), row.mass[b]};
-      else cut = resolve(b, (unsigned)k - row.before(b), 0.0, false, ~0u, order);
+      else cut = resolve(b, (unsigned)k - row.before(b), 0.0, false, ~0u, n_list, order);
     }
     if (use_p) {
       const double want = (double)p * cut.mass;
       const int b = row.find_mass(want, false);
-      if (b < cut.bucket || (b == cut.bucket && cut.count > 0)) cut = resolve(b, 0, want, false, b < cut.bucket ? ~0u : cut.count, order);
+      if (b < cut.bucket || (b == cut.bucket && cut.count > 0)) cut = resolve(b, 0, want, false, b < cut.bucket ? ~0u : cut.count, n_list, order);
     }
     if (use_least && least_bucket <= cut.bucket) {
-      ask({kCountLeast, least_bucket, least_bucket, 0, 0});
-      const unsigned in = (unsigned)sh.counted, has = row.count[least_bucket] - row.before(least_bucket);
+      const unsigned has = row.count[least_bucket] - row.before(least_bucket);
+      unsigned in = 0;
+      if (n_list) {
+        if (has) {
+          const int from = first_of(n_list, [&](int i) { return scale.bucket(value_of(sh.list[i])) >= least_bucket; });
+          in = first_of((int)has + 1, [&](int i) { return i == (int)has || !reaches_least(value_of(sh.list[from + i])); });
+        }
+      } else {
+        ask({kCountLeast, least_bucket, least_bucket, 0, 0, 0, {}, {}});
+        in = (unsigned)sh.counted;
+      }
       if (least_bucket < cut.bucket || in < cut.count) {
         if (in == 0) cut = {least_bucket, 0, row.mass_before(least_bucket)};
         else if (in == has) cut = {least_bucket, in, row.mass[least_bucket]};
-        else cut = resolve(least_bucket, in, 0.0, false, ~0u, order);
+        else cut = resolve(least_bucket, in, 0.0, false, ~0u, n_list, order);
       }
     }
     total = cut.mass;
     const double want = draw * total;
     int b = row.find_mass(want, true);
     if (b < cut.bucket || (b == cut.bucket && cut.count > 0)) {
-      resolve(b, 0, want, true, b < cut.bucket ? ~0u : cut.count, order);
+      resolve(b, 0, want, true, b < cut.bucket ? ~0u : cut.count, n_list, order);
     } else {  // the draw fell behind the cut by a rounding: the last one kept
       const unsigned kept = row.before(cut.bucket) + cut.count;
       b = row.find_count(kept);
-      resolve(b, kept - row.before(b), 0.0, false, ~0u, order);
+      // its bucket need not be among those that are listed
+      resolve(b, kept - row.before(b), 0.0, false, ~0u, 0, order);
     }
   }
 };
@@ -735,7 +819,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice
   r.scale = Scale(r.seen(value_of(best)), t);
   r.temperature = t;
   r.least = a.min_p ? __ldg(a.min_p + row) : 0.0f;
-  r.template add_up<false>({kHistogram, 0, kBuckets - 1, 0, 0});
+  r.template add_up<false>({kHistogram, 0, kBuckets - 1, 0, 0, 0, {}, {}});
   r.share_sums();
   if (rank == 0) {
     u64 order = best;
@@ -746,13 +830,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice
       // the best token may be +infinity, which the sums see as 0; its weight is 1 in any case
       if (a.probs) a.probs[row] = order == best ? (float)(1.0 / total) : (float)(r.scale.weight(value_of(order)) / total);
     }
-    if (kCl > 1) r.ask({kDone, 0, 0, 0, 0});
+    if (kCl > 1) r.ask({kDone, 0, 0, 0, 0, 0, {}, {}});
   } else {
     for (;;) {
       r.sync_all();
-      const Command cmd = sh.command;
-      if (cmd.op == kDone) break;
-      r.serve(cmd);
+      if (sh.command.op == kDone) break;
+      r.serve();
       r.sync_all();
     }
   }
