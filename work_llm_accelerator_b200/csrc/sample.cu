@@ -12,8 +12,8 @@
 // random: f is exact to 2^-30, which a drawn number that falls between 150000 small weights needs.
 //
 // A row is read three times: for its maximum, for the bucket sums, for the tokens to sort; the second and third
-// reading mostly meet L2. A cluster of 8 CTAs shares a row, fewer when there are rows enough to fill the GPU with
-// two CTAs per SM. The first CTA leads: it reads the others' bucket sums through distributed shared memory, decides
+// reading mostly meet L2. A cluster of 8 CTAs shares a row while all of them find an SM of their own, and of 4, 2 or 1 while all of
+// them run at once, two per SM. The first CTA leads: it reads the others' bucket sums through distributed shared memory, decides
 // (every thread the same way, by bisection, without barriers) and asks for what it needs to see. Bound: for few rows
 // the latency of those steps, for many the ~35 instructions and two shared atomics per logit of the second pass.
 #include <cooperative_groups.h>
@@ -39,11 +39,10 @@ constexpr int kList = 2048;  // tokens that are sorted at once
 constexpr int kOrderBits = 50;
 constexpr int kDigit = 11;        // bits by which a crowded bucket is narrowed at a time
 constexpr int kFold = 1 << 15;    // logits whose q, below 2^17 each, fit a 32-bit sum
-constexpr int kLight = 8;         // 16-byte loads that a thread has under way in the passes that only compare
-constexpr int kHeavy = 4;         // and in the pass that sums
+constexpr int kAhead = 4;         // 16-byte loads that a thread has under way (8 cost registers: 256 rows took 9% longer)
 constexpr int kMaxCluster = 8;
 constexpr int kOneCta = 8192;     // vocabularies up to this size take one CTA: less to read than a cluster costs to sync
-constexpr int kResident = 2 * 148;  // CTAs that fit the GPU at once
+constexpr int kSms = 148;
 
 typedef unsigned long long u64;
 
@@ -278,7 +277,7 @@ struct Row {
 
   // f(values, number of them, place of the first) for places from .. to - 1 of this CTA's logits: 16-byte loads, a few
   // at a time, between the first and the last aligned place, single ones outside.
-  template <int kAhead, typename F>
+  template <int kMany, typename F>
   __device__ __forceinline__ void for_each(int from, int to, F f) {
     constexpr int kVec = V::kVec;
     const int head = min(to - from, (int)((16 - reinterpret_cast<uintptr_t>(x + from) % 16) % 16 / sizeof(T)));
@@ -290,18 +289,18 @@ struct Row {
     }
     const uint4* v = reinterpret_cast<const uint4*>(x + from + head) + threadIdx.x;
     int at = from + head + (int)threadIdx.x * kVec, left = vecs - (int)threadIdx.x;
-    for (; left > (kAhead - 1) * kThreads; left -= kAhead * kThreads) {
-      uint4 b[kAhead];
+    for (; left > (kMany - 1) * kThreads; left -= kMany * kThreads) {
+      uint4 b[kMany];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) b[k] = __ldg(v + k * kThreads);
+      for (int k = 0; k < kMany; ++k) b[k] = __ldg(v + k * kThreads);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
+      for (int k = 0; k < kMany; ++k) {
         float e[kVec];
         V::unpack(b[k], e);
         f(e, at + k * kThreads * kVec);
       }
-      v += kAhead * kThreads;
-      at += kAhead * kThreads * kVec;
+      v += kMany * kThreads;
+      at += kMany * kThreads * kVec;
     }
     for (; left > 0; left -= kThreads) {
       float e[kVec];
@@ -333,7 +332,7 @@ struct Row {
     const unsigned hist = (unsigned)__cvta_generic_to_shared(&sh.hist[0][0]) - 4 * __float_as_uint(Scale::kFloor);
     for (int from = 0; from < max(n, 1); from += kFold) {
       clear_histogram();
-      for_each<kHeavy>(from, min(n, from + kFold), [&](const auto& e, int at) {
+      for_each<kAhead>(from, min(n, from + kFold), [&](const auto& e, int at) {
         constexpr int kN = (int)(sizeof(e) / sizeof(float));
         float v[kN];
 #pragma unroll
@@ -407,7 +406,7 @@ struct Row {
         from[k] = k < cmd.ranges ? (float)cmd.from[k] : 1.0f;
         end[k] = k < cmd.ranges ? (float)(cmd.to[k] + 1) : 0.0f;
       }
-      for_each<kLight / 2>(0, n, [&](const auto& e, int at) {
+      for_each<kAhead>(0, n, [&](const auto& e, int at) {
         constexpr int kN = (int)(sizeof(e) / sizeof(float));
         unsigned in = 0;
 #pragma unroll
@@ -429,7 +428,7 @@ struct Row {
       const float a = sc.top - end / sc.c, b = sc.top - from / sc.c;
       const float wide = (fabsf(sc.top) + fmaxf(fabsf(a), fabsf(b))) * 1e-6f;
       const float v_low = a - wide, v_high = b + wide;  // NaN or infinite: every logit is looked at
-      for_each<kLight>(0, n, [&](const auto& e, int at) {
+      for_each<kAhead>(0, n, [&](const auto& e, int at) {
         constexpr int kN = (int)(sizeof(e) / sizeof(float));
         bool any = infinite;
 #pragma unroll
@@ -768,8 +767,9 @@ struct Row {
   }
 };
 
+// A cluster of 8 has its SMs to itself and takes the registers that the leader's part wants (1 row: 18.3 us, 20.9 with 64).
 template <int kType, int kCl>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice) {
+__global__ void __launch_bounds__(kThreads, kCl == kMaxCluster ? 1 : 2) sample_kernel(Sample a, int slice) {
   using R = Row<kType, kCl>;
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Sample a, int slice
 
   float top = -INFINITY;
   int top_at = 0;
-  r.template for_each<kLight>(0, r.n, [&](const auto& e, int at) {
+  r.template for_each<kAhead>(0, r.n, [&](const auto& e, int at) {
     float m = e[0];
 #pragma unroll
     for (int i = 1; i < (int)(sizeof(e) / sizeof(float)); ++i) m = fmaxf(m, e[i]);
@@ -862,9 +862,10 @@ cudaError_t launch(const Sample& a, cudaStream_t s) {
 
 template <int kType>
 cudaError_t launch(const Sample& a, cudaStream_t s) {
-  if (a.vocab <= kOneCta || a.rows * 2 > kResident) return launch<kType, 1>(a, s);
-  if (a.rows * 4 > kResident) return launch<kType, 2>(a, s);
-  return a.rows * 8 > kResident ? launch<kType, 4>(a, s) : launch<kType, 8>(a, s);
+  const long long rows = a.rows;
+  if (a.vocab <= kOneCta || rows * 2 > 2 * kSms) return launch<kType, 1>(a, s);
+  if (rows * 4 > 2 * kSms) return launch<kType, 2>(a, s);
+  return rows * 8 > kSms ? launch<kType, 4>(a, s) : launch<kType, 8>(a, s);
 }
 
 }  // namespace
