@@ -347,6 +347,33 @@ def test_attention_long_and_many(n, length):
     check_rows(c, q, "f32", list(range(n)), lens, out, lse)
 
 
+@pytest.mark.parametrize("n,length", [(60, 1100), (70, 700), (148, 64)])
+def test_attention_equal_lengths(n, length):
+    """Batches whose sequences are alike: each fits a CTA's share of the work or nearly does."""
+    import torch
+
+    lens = [length] * n
+    c = filled(lens, 2, seed=n)
+    q = torch.randn(n, 12, 128, generator=torch.Generator().manual_seed(n)).cuda()
+    out, lse, _ = attend(c, q, "f32", ints(range(n)), ints(lens))
+    check_rows(c, q, "f32", list(range(n)), lens, out, lse)
+
+
+def test_attention_workspace_is_used_again():
+    """Calls of other shapes, one after the other in one workspace, leave nothing behind that a later one takes up."""
+    import torch
+
+    lens = [9000, 700, 2500]
+    c = filled(lens, 2, seed=71)
+    q = torch.randn(3, 12, 128, generator=torch.Generator().manual_seed(9)).cuda()
+    work = None
+    for rows in ([0], [1, 2], [0, 1, 2], [2], [0], [0, 1, 2]):
+        ns = [lens[r] - 3 for r in rows]
+        out, lse, work = attend(c, q[rows], "f32", ints(rows), ints(ns), work=work)
+        torch.cuda.synchronize()
+        check_rows(c, q[rows], "f32", rows, ns, out, lse)
+
+
 def test_attention_drafts_padded_rows_and_strides():
     """Several rows of one sequence with rising lengths, rows without a sequence, q inside a wider row, out too."""
     import torch

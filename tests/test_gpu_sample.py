@@ -164,6 +164,20 @@ def test_two_levels_of_ties():
         assert got[0] == ids[at], at
 
 
+@pytest.mark.parametrize("rows", [18, 19, 40, 75, 150])
+def test_row_counts_that_share_the_gpu_differently(rows):
+    """Ties by the thousand and ordinary rows, at numbers of rows that give a row 8, 4, 2 CTAs and one."""
+    import torch
+
+    x = gaussian(rows, 20000, "f32", rows)
+    x[::2] = 0.5  # every second row: all equal
+    k = [[0, 12000, 700][i % 3] for i in range(rows)]
+    check(x, "f32", rows, temperature=[0.9] * rows, top_k=k)
+    js = [i * 7 % 600 for i in range(rows)]
+    got, _ = run(x[::2], [(j + 0.5) / 12000 for j in js][: len(x[::2])], top_k=[12000] * len(x[::2]))
+    assert list(got) == js[: len(got)]
+
+
 @pytest.mark.parametrize("spread", [1e-6, 1e-3, 0.05])
 def test_crowded_logits(spread):
     """All logits within a narrow band: thousands share what a coarse view would call one value."""

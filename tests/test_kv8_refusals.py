@@ -65,6 +65,10 @@ def test_attention_refusals(host):
                      (dict(row_seqs_ptr=0), "row_seqs is null"), (dict(row_lens_ptr=A + 2), "row_lens is not"),
                      (dict(lse_ptr=A + 1), "lse is not")]:
         refused(host, lambda: host.kv8_attention(cache(host), **{**good, **kw}), text)
+    big = dict(n_rows=1 << 20, workspace_bytes=1 << 40)
+    wide = dict(n_q_heads=64, q_stride=8192, out_stride=8192)
+    refused(host, lambda: host.kv8_attention(cache(host, max_blocks=1 << 24), **{**good, **wide}), "n_q_heads * max_blocks")
+    refused(host, lambda: host.kv8_attention(cache(host, max_blocks=1 << 16), **{**good, **big}), "n_rows * n_q_heads * max_blocks")
     host.kv8_attention(cache(host), **{**good, "n_rows": 0})
     for args in ((-1, 12, 2), (1, 0, 2), (1, 12, 0)):
         with pytest.raises(host.EngineError):

@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
   }
   __syncthreads();
   const long long cta0 = border[0];
-  const int cta_n = (int)(border[1] - cta0);  // the entry point bounds all by 2^40
+  const int cta_n = (int)(border[1] - cta0);  // the entry point bounds all by 2^37
   const int per_warp = (cta_n + kWarps - 1) / kWarps;
   if (mine > 0 && before < cta0 + cta_n && before + mine > cta0) {
     long long pos = before;

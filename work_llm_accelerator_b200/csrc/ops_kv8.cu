@@ -168,10 +168,10 @@ extern "C" int qwen_b200_kv8_attention(const qwen_b200_kv8_cache* cache, const v
     set_error("%s: n_q_heads %d is not a multiple of n_kv_heads %d", op, n_q_heads, cache->n_kv_heads);
     return kStatusInvalid;
   }
-  // items and a row's tiles are counted in 31 bits, all tiles in 40
+  // items, a row's tiles and a CTA's share of all tiles are counted in 31 bits
   if (!range_ok(op, "n_q_heads * max_blocks", (long long)n_q_heads * cache->max_blocks, 0, 1ll << 29) ||
       !range_ok(op, "n_rows * n_q_heads", (long long)n_rows * n_q_heads, 0, 1ll << 29) ||
-      !range_ok(op, "n_rows * n_q_heads * max_blocks", (long long)n_rows * n_q_heads * cache->max_blocks, 0, 1ll << 39))
+      !range_ok(op, "n_rows * n_q_heads * max_blocks", (long long)n_rows * n_q_heads * cache->max_blocks, 0, 1ll << 36))
     return kStatusInvalid;
   if (!std::isfinite(scale)) {
     set_error("%s: scale is not finite", op);
