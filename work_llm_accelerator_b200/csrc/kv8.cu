@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, void* k, void* 
   for (int i = 0; i < kSlotsPerWarp; ++i) {
     const int t = warp + i * kWarps;
     if (t >= w.n) break;
-    store4(x + t * r.stride, values_of(kb[i], ks));
-    store4(y + t * r.stride, values_of(vb[i], vs));
+    stream4(x + t * r.stride, values_of(kb[i], ks));
+    stream4(y + t * r.stride, values_of(vb[i], vs));
   }
 }
 

@@ -56,5 +56,15 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = b;
 }
 
+// The same for values that are not read again soon: evicted first, the cache keeps what is (reading 8 x 4096 rows back:
+// 17.6 us without, 16.9 us with).
+__device__ __forceinline__ void stream4(float* p, float4 v) { __stcs(reinterpret_cast<float4*>(p), v); }
+template <typename T>
+__device__ __forceinline__ void stream4(T* p, float4 v) {
+  __align__(8) T four[4];
+  store4(four, v);
+  __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<const uint2*>(four));
+}
+
 }  // namespace kv8
 }  // namespace qb
