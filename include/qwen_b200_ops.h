@@ -95,8 +95,10 @@ enum { QWEN_B200_F32 = 0, QWEN_B200_F16 = 1, QWEN_B200_BF16 = 2 };
  *   k_scales, v_scales  [n_blocks][n_kv_heads] fp32
  *   block_table         [n_seqs][max_blocks] int32: token t of sequence s is slot t % 64 of block
  *                       block_table[s][t / 64]; entries behind a sequence's last block are not read
- * Blocks need no initialisation. Indexes that live on the device are checked there: a kernel that meets one outside
- * of its buffers skips the access and sets bit 1 of qwen_b200_kernel_error(); values of such a place read as NaN. */
+ * Blocks need no initialisation. Indexes that live on the device are checked there; a kernel that meets one outside of
+ * its buffers touches nothing there and sets bit 1 of qwen_b200_kernel_error(): a block id reads as NaN and is not
+ * written, a segment whose sequence, positions or rows lie outside is left out, and an attention row whose sequence or
+ * length does is NaN. */
 typedef struct qwen_b200_kv8_cache {
   signed char* k_codes;
   signed char* v_codes;
@@ -128,7 +130,7 @@ int qwen_b200_kv8_append(const qwen_b200_kv8_cache* cache, const void* k, const 
                          const int* offsets, int n_segments, void* stream);
 
 /* Read cached rows back: segment i writes tokens starts[i] .. of sequence seqs[i] to rows offsets[i] ..
- * offsets[i + 1] - 1 of k and v, as code * scale rounded to `dtype`. Arguments as above; rows from
+ * offsets[i + 1] - 1 of k and v (different buffers), as code * scale rounded to `dtype`. Arguments as above; rows from
  * offsets[n_segments] on are left as they are, and a sequence may be named more than once. */
 int qwen_b200_kv8_read(const qwen_b200_kv8_cache* cache, void* k, void* v, int dtype, long long row_stride,
                        long long n_rows, const int* seqs, const int* starts, const int* offsets, int n_segments,
@@ -161,7 +163,9 @@ long long qwen_b200_kv8_attention_workspace(int n_rows, int n_q_heads, int n_kv_
  *   min_p > 0  keeps those of w >= min_p (the first one in any case);
  * the token is the first whose running sum of w exceeds uniform * (sum of the kept w), the last one kept if none does.
  * temperature below 2^-126 (0 included) or NaN: the first token, with probability 1. Logits of -infinity or NaN are
- * never taken; a row without any other gives token -1, probability 0. +infinity outweighs every finite logit.
+ * never taken; a row without any other gives token -1, probability 0. +infinity outweighs every finite logit. Weights
+ * below exp(-32) of the largest count as 0; the others are within (2 + z) 2^-24 of themselves, z = (max - logit) /
+ * temperature.
  *   logits      [rows][vocab] of `dtype`, rows row_stride elements apart; 1 <= vocab <= 262144
  *   temperature, top_k, top_p, min_p  [rows] fp32 / int32, or NULL (1, off, off, off)
  *   uniforms    [rows] fp32 in [0, 1)

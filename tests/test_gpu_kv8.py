@@ -374,6 +374,29 @@ def test_attention_workspace_is_used_again():
         check_rows(c, q[rows], "f32", rows, ns, out, lse)
 
 
+def test_attention_two_graphs_share_a_workspace():
+    """Two captured calls with one workspace, replayed in turn: each finds what the other left."""
+    import torch
+
+    lens = [9000, 4000]
+    c = filled(lens, 2, seed=72)
+    shapes = [([0, 1], [9000, 4000]), ([0], [8000])]
+    qs = [torch.randn(len(s), 12, 128, generator=torch.Generator().manual_seed(i)).cuda() for i, (s, _) in enumerate(shapes)]
+    idx = [(ints(s), ints(n)) for s, n in shapes]
+    outs, lses, graphs = [torch.full_like(q, 7.0) for q in qs], [torch.full(q.shape[:2], 7.0, device="cuda") for q in qs], []
+    _, _, work = attend(c, qs[0], "f32", *idx[0])
+    torch.cuda.synchronize()
+    for i, q in enumerate(qs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            attend(c, q, "f32", *idx[i], out=outs[i], lse=lses[i], work=work)
+    for turn in (0, 1, 0, 0, 1, 1, 0):
+        outs[turn].fill_(7.0)
+        graphs[turn].replay()
+        torch.cuda.synchronize()
+        check_rows(c, qs[turn], "f32", *shapes[turn], outs[turn], lses[turn])
+
+
 def test_attention_drafts_padded_rows_and_strides():
     """Several rows of one sequence with rising lengths, rows without a sequence, q inside a wider row, out too."""
     import torch

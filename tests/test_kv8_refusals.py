@@ -38,7 +38,7 @@ def refused(host, call, text):
 @pytest.mark.parametrize("name", ["kv8_append", "kv8_read"])
 def test_rows_refusals(host, name):
     fn = getattr(host, name)
-    good = dict(k_ptr=A, v_ptr=A, dtype=0, row_stride=256, n_rows=3, seqs_ptr=A, starts_ptr=A, offsets_ptr=A, n_segments=1)
+    good = dict(k_ptr=A, v_ptr=A if name == "kv8_append" else 2 * A, dtype=0, row_stride=256, n_rows=3, seqs_ptr=A, starts_ptr=A, offsets_ptr=A, n_segments=1)
     for kw, text in CACHE:
         refused(host, lambda: fn(cache(host, **kw), **good), text)
     for kw, text in [(dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(row_stride=255), "row_stride"),
@@ -47,6 +47,8 @@ def test_rows_refusals(host, name):
                      (dict(v_ptr=A + 4), "v is not 16-byte"), (dict(seqs_ptr=0), "seqs is null"),
                      (dict(starts_ptr=A + 1), "starts is not 4-byte"), (dict(offsets_ptr=0), "offsets is null")]:
         refused(host, lambda: fn(cache(host), **{**good, **kw}), text)
+    if name == "kv8_read":
+        refused(host, lambda: fn(cache(host), **{**good, "v_ptr": A}), "one buffer")
     fn(cache(host), **{**good, "n_rows": 0})  # nothing to do: no error, no GPU
     fn(cache(host), **{**good, "n_segments": 0})
 
@@ -69,7 +71,7 @@ def test_attention_refusals(host):
     wide = dict(n_q_heads=64, q_stride=8192, out_stride=8192)
     refused(host, lambda: host.kv8_attention(cache(host, max_blocks=1 << 24), **{**good, **wide}), "n_q_heads * max_blocks")
     refused(host, lambda: host.kv8_attention(cache(host, max_blocks=1 << 16), **{**good, **big}), "n_rows * n_q_heads * max_blocks")
-    host.kv8_attention(cache(host), **{**good, "n_rows": 0})
+    host.kv8_attention(cache(host), **{**good, "n_rows": 0, "workspace_bytes": 0})
     for args in ((-1, 12, 2), (1, 0, 2), (1, 12, 0)):
         with pytest.raises(host.EngineError):
             host.kv8_attention_workspace(*args)
@@ -90,14 +92,14 @@ def test_sample_refusals(host):
 
 def test_without_a_device_or_with_host_memory(host, gpu_available):
     """Sound arguments on a machine without a GPU: status 31 (host memory on one with a GPU: status 1); never computed."""
-    x = np.zeros(4096, np.float32)
+    x = np.zeros(8192, np.float32)
     p = x.ctypes.data // 16 * 16 + 16
     c = cache(host, k_codes_ptr=p, v_codes_ptr=p, k_scales_ptr=p, v_scales_ptr=p, block_table_ptr=p)
     want = "status 1:" if gpu_available else "status 31:"
     with pytest.raises(host.EngineError, match=want):
         host.kv8_append(c, p, p, 0, 256, 1, p, p, p, 1)
     with pytest.raises(host.EngineError, match=want):
-        host.kv8_read(c, p, p, 0, 256, 1, p, p, p, 1)
+        host.kv8_read(c, p, p + 4096, 0, 256, 1, p, p, p, 1)
     with pytest.raises(host.EngineError, match=want):
         host.kv8_attention(c, p, 1536, p + 16, 1536, 0, 1, 12, p, p, 0.1, p, 1 << 30)
     with pytest.raises(host.EngineError, match=want):

@@ -3,7 +3,9 @@
 // One CTA takes one block of 64 tokens of one sequence and kv head: a block has one scale, so the CTA that owns
 // it sees every value that the scale depends on and no two CTAs write the same bytes. Both kernels are bound by
 // the bytes they move, small calls by the chain of loads that finds a CTA's block (segments, block table, data); each
-// value is loaded once, kept in registers while the CTA agrees on the scales, and stored once.
+// value is loaded once, kept in registers while the CTA agrees on the scale, and stored once.
+// Measured on B200, 2 kv heads: append of 64 single rows 3.3 us, of 4096 fp32 rows 4.1 us, of 18400 bf16 rows in ragged
+// chunks 10.1 us (28 MB); read of 32768 fp32 rows 16.9 us (84 MB, 5.0 TB/s).
 #include <cuda_runtime.h>
 
 #include "kv8_device.cuh"
@@ -113,10 +115,10 @@ __device__ __forceinline__ unsigned abs_bits(float4 v) {
              max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
 }
 
-// K and V in CTAs of their own: with both in one, its registers leave room for two CTAs per SM and 18400 rows took 16.2 us
-// instead of 11.7.
+// K and V in CTAs of their own, 16-bit values packed until they are used: with both in one CTA, its registers leave room
+// for two per SM and 18400 bf16 rows took 16.2 us; apart 11.7, packed 10.1.
 template <int kType>
-__global__ void __launch_bounds__(kThreads, 4) append_kernel(Cache c, const void* k, const void* v, Rows r) {
+__global__ void __launch_bounds__(kThreads, kType == 0 ? 4 : kType == 1 ? 5 : 6) append_kernel(Cache c, const void* k, const void* v, Rows r) {
   using T = typename TypeOf<kType>::T;
   __shared__ unsigned warp_max[kWarps];
   Work w;
@@ -129,15 +131,16 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(Cache c, const void
   const bool opened = w.first_slot > 0;
   const float old = opened ? *scale : 0.0f;
 
-  float4 val[kSlotsPerWarp];
+  decltype(raw4(x)) val[kSlotsPerWarp];
 #pragma unroll
   for (int i = 0; i < kSlotsPerWarp; ++i) {
     const int t = warp + i * kWarps;
-    val[i] = t < w.n ? load4(x + t * r.stride) : make_float4(0.f, 0.f, 0.f, 0.f);
+    val[i] = {};
+    if (t < w.n) val[i] = raw4(x + t * r.stride);
   }
   unsigned a = 0;  // absolute values compare as their bits; NaN and infinities are the largest
 #pragma unroll
-  for (int i = 0; i < kSlotsPerWarp; ++i) a = max(a, abs_bits(val[i]));
+  for (int i = 0; i < kSlotsPerWarp; ++i) a = max(a, abs_bits(expand<T>(val[i])));
   a = __reduce_max_sync(0xffffffffu, a);
   if (lane == 0) warp_max[warp] = a;
   __syncthreads();
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(Cache c, const void
   codes += (w.first_slot + warp) * (kHead / 4);
 #pragma unroll
   for (int i = 0; i < kSlotsPerWarp; ++i)
-    if (warp + i * kWarps < w.n) codes[i * kWarps * (kHead / 4)] = zero ? 0 : codes_of(val[i], s, inv);
+    if (warp + i * kWarps < w.n) codes[i * kWarps * (kHead / 4)] = zero ? 0 : codes_of(expand<T>(val[i]), s, inv);
 }
 
 __device__ __forceinline__ float4 values_of(int b, float s) {

@@ -13,7 +13,6 @@ namespace kv8 {
 
 constexpr int kBlock = 64;    // tokens of a block (the engine's page, kPage)
 constexpr int kHead = 128;    // head dimension
-constexpr int kTypes = 3;     // 0 fp32, 1 fp16, 2 bf16
 
 struct Cache {
   int8_t* codes[2];    // K, V: [n_blocks][heads][64][128]
@@ -30,6 +29,7 @@ struct Rows {
   long long stride;  // elements from row to row
 };
 
+// `type`: 0 fp32, 1 fp16, 2 bf16.
 cudaError_t launch_append(const Cache& c, const void* k, const void* v, int type, const Rows& r, cudaStream_t s);
 cudaError_t launch_read(const Cache& c, void* k, void* v, int type, const Rows& r, cudaStream_t s);
 

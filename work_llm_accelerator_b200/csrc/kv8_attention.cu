@@ -12,7 +12,10 @@
 // Each tile is joined to the running maximum and sums in fp32, so weights that are small beside another tile's keep
 // their bits.
 //
-// Bound: HBM bytes of the cache (256 + 8/64 per token and kv head).
+// Bound: HBM bytes of the cache (256 + 8/64 per token and kv head). Measured on B200 (12 heads on 2): 64 sequences x 2048
+// 21.1 us (67.7 MB, 3.2 TB/s; loads alone 18.1, arithmetic alone 18.1, two warps per scheduler hide either only in
+// part), 1 x 131072 32.1 us, 1 x 517 10.3 us. On fp16 halves (m16n8k16) the codes' conversion cost 350 instructions per
+// tile where the digits cost 64, and 64 x 2048 took 27.5 us; tensor-map loads instead of cp.async gave 21.6.
 //
 // Split: all (row, kv head) items lie end to end as tiles, in equal runs over the CTAs and in each CTA over its warps,
 // whatever the lengths are; a border that would cut an item moves to its beginning where that makes no run much longer.

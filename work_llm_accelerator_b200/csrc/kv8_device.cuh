@@ -25,20 +25,36 @@ struct TypeOf<2> {
   using T = __nv_bfloat16;
 };
 
+template <typename T>
+constexpr bool kIsBf16 = false;
+template <>
+constexpr bool kIsBf16<__nv_bfloat16> = true;
+
 __device__ __forceinline__ void bad_index() { atomicOr(&g_kernel_error, kErrBadIndex); }
 
-// Four consecutive values as fp32. The entry points check the alignment (four values: 16 or 8 bytes).
-__device__ __forceinline__ float4 load4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
-__device__ __forceinline__ float4 load4(const __half* p) {
-  const uint2 b = __ldg(reinterpret_cast<const uint2*>(p));
-  const float2 lo = __half22float2(reinterpret_cast<const __half2&>(b.x));
-  const float2 hi = __half22float2(reinterpret_cast<const __half2&>(b.y));
-  return make_float4(lo.x, lo.y, hi.x, hi.y);
+// Four consecutive values as they lie in memory, and as fp32. The entry points check the alignment (16 or 8 bytes).
+__device__ __forceinline__ float4 raw4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+template <typename T>
+__device__ __forceinline__ uint2 raw4(const T* p) {
+  return __ldg(reinterpret_cast<const uint2*>(p));
 }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 b = __ldg(reinterpret_cast<const uint2*>(p));
+template <typename T>
+__device__ __forceinline__ float4 expand(float4 b) {
+  return b;
+}
+template <typename T>
+__device__ __forceinline__ float4 expand(uint2 b) {
+  if (sizeof(T) == 2 && !kIsBf16<T>) {
+    const float2 lo = __half22float2(reinterpret_cast<const __half2&>(b.x));
+    const float2 hi = __half22float2(reinterpret_cast<const __half2&>(b.y));
+    return make_float4(lo.x, lo.y, hi.x, hi.y);
+  }
   return make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16),
                      __uint_as_float(b.y & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  return expand<T>(raw4(p));
 }
 
 // The rounding to the caller's type: the one rounding of a value that was computed in fp32.

@@ -1,6 +1,8 @@
 // Entry points of the 8-bit KV cache operators and of token sampling (include/qwen_b200_ops.h): the argument
 // checks that the host can make, then one launch on the caller's stream. Nothing here allocates or synchronises,
 // so every call can be captured into a graph.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -29,6 +31,34 @@ bool range_ok(const char* op, const char* name, long long v, long long lo, long 
   return false;
 }
 
+// Memory of device `dev`, or managed memory. The driver's own query takes half of the runtime's time, and a call asks for
+// up to eleven buffers; where it cannot be had, the runtime answers.
+bool on_device(const void* p, int dev) {
+  static const PFN_cuPointerGetAttributes_v7000 query = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    return cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &r) == cudaSuccess &&
+                   r == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<PFN_cuPointerGetAttributes_v7000>(f)
+               : nullptr;
+  }();
+  if (query) {
+    unsigned type = 0, managed = 0;  // a type of 0: not known to CUDA
+    int ordinal = -1;
+    CUpointer_attribute names[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL,
+                                    CU_POINTER_ATTRIBUTE_IS_MANAGED};
+    void* values[3] = {&type, &ordinal, &managed};
+    return query(3, names, values, reinterpret_cast<CUdeviceptr>(p)) == CUDA_SUCCESS &&
+           (managed || (type == CU_MEMORYTYPE_DEVICE && ordinal == dev));
+  }
+  cudaPointerAttributes a;
+  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeDevice && a.device == dev);
+}
+
 // Every buffer: present, aligned, and memory of the current device (or managed memory).
 int check_buffers(const char* op, const Arg* args, int n) {
   for (int i = 0; i < n; ++i) {
@@ -48,12 +78,7 @@ int check_buffers(const char* op, const Arg* args, int n) {
     return kStatusNoDevice;
   }
   for (int i = 0; i < n; ++i) {
-    cudaPointerAttributes a;
-    if (cudaPointerGetAttributes(&a, args[i].p) != cudaSuccess) {
-      cudaGetLastError();
-      a.type = cudaMemoryTypeUnregistered;
-    }
-    if (a.type != cudaMemoryTypeManaged && !(a.type == cudaMemoryTypeDevice && a.device == dev)) {
+    if (!on_device(args[i].p, dev)) {
       set_error("%s: %s must be memory of the current device (%d) or managed memory", op, args[i].name, dev);
       return kStatusInvalid;
     }
@@ -110,6 +135,10 @@ int rows_call(const char* op, const qwen_b200_kv8_cache* c, const void* k, const
       !stride_ok(op, "row_stride", row_stride, (long long)c->n_kv_heads * kv8::kHead, dtype))
     return kStatusInvalid;
   if (n_rows == 0 || n_segments == 0) return 0;
+  if (!kWrite && k == v && k) {
+    set_error("%s: k and v are one buffer", op);
+    return kStatusInvalid;
+  }
   const Arg args[] = {{"k", k, 16},
                       {"v", v, 16},
                       {"k_codes", c->k_codes, 16},
@@ -177,6 +206,7 @@ extern "C" int qwen_b200_kv8_attention(const qwen_b200_kv8_cache* cache, const v
     set_error("%s: scale is not finite", op);
     return kStatusInvalid;
   }
+  if (n_rows == 0) return 0;
   const long long need = (long long)kv8::attention_workspace(n_rows, n_q_heads, cache->n_kv_heads);
   if (workspace_bytes < need) {
     set_error("%s: workspace of %lld bytes, %lld needed", op, workspace_bytes, need);
@@ -186,7 +216,6 @@ extern "C" int qwen_b200_kv8_attention(const qwen_b200_kv8_cache* cache, const v
     set_error("%s: out is q; they must not overlap", op);
     return kStatusInvalid;
   }
-  if (n_rows == 0) return 0;
   const Arg args[] = {{"q", q, 16},
                       {"out", out, 16},
                       {"k_codes", cache->k_codes, 16},
