@@ -14,7 +14,7 @@
 //
 // Bound: HBM bytes of the cache (256 + 8/64 per token and kv head). Measured on B200 (12 heads on 2): 64 sequences x 2048
 // 21.1 us (67.7 MB, 3.2 TB/s; loads alone 18.1, arithmetic alone 18.1, two warps per scheduler hide either only in
-// part), 1 x 131072 32.1 us, 1 x 517 10.3 us. On fp16 halves (m16n8k16) the codes' conversion cost 350 instructions per
+// part), 1 x 131072 29.5 us, 1 x 517 10.1 us. On fp16 halves (m16n8k16) the codes' conversion cost 350 instructions per
 // tile where the digits cost 64, and 64 x 2048 took 27.5 us; tensor-map loads instead of cp.async gave 21.6.
 //
 // Split: all (row, kv head) items lie end to end as tiles, in equal runs over the CTAs and in each CTA over its warps,
@@ -85,10 +85,11 @@ __device__ __forceinline__ bool all_parts(u64* flags, u64 call, int mine, int n)
     all = all && x == call;
   }
   all = __all_sync(0xffffffffu, all);
-  if (all)
+  if (all) {
     for (int i = lane; i < n; i += 32)
       asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(flags + (i ? 2 * i - 1 : 0)), "l"(0ull) : "memory");
-  __threadfence();
+    __threadfence();  // the parts are read behind the flags
+  }
   return all;
 }
 
@@ -228,7 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
   __shared__ long long warp_sum[kWarps], part_from[kWarps], border[2];
   __shared__ unsigned warp_least[kWarps], warp_most[kWarps];
   __shared__ int4 start[kWarps];  // row, first tile among the row's, length, sequence
-  __shared__ int part_item[2 * kWarps], part_ended[kWarps], is_last;
+  __shared__ int part_item[2 * kWarps], part_ended[kWarps];
+  __shared__ int2 join[2];  // an item whose parts are joined here: its first CTA, and how many have a part
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q4 = lane % 4;
 
   // ---- the runs: tiles before each thread's rows, the whole, and where this CTA's warps begin
@@ -644,25 +646,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
     }
   }
 
-  // ---- join an item's parts over the CTAs, in the one that finishes last
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const int item = open_item[which];
-    if (item < 0) continue;  // the same for all threads
-    const int it_row = item / lay.subs, it_sub = item - it_row * lay.subs;
-    // the item's tiles begin at `from`: in which CTA, and in how many
-    const int tiles = row_tiles(c, a, it_row);
-    const long long from = which ? part_from[after_warp] : cta0 - start[0].y % tiles;
-    const int first_cta = run_of(from, per_cta), n = run_of(from + tiles - 1, per_cta) - first_cta + 1;
+  // ---- join an item's parts over the CTAs, in the one that finishes last: a CTA has a part of at most two
+  if (open_item[0] >= 0 || open_item[1] >= 0) {
     __syncthreads();
-    if (warp == 0) {
-      // the item's flags: that of part 2 first_cta + 1, then of every second one
-      u64* flags = reinterpret_cast<u64*>(static_cast<uint8_t*>(a.work) + kFlagsOffset) + 2 * first_cta + 1;
-      const bool last = all_parts(flags, call, (int)blockIdx.x - first_cta, n);
-      if (lane == 0) is_last = last;
+    if (warp < 2) {
+      const int item = warp ? open_item[1] : open_item[0];
+      bool last = false;
+      if (item >= 0) {
+        // the item's tiles begin at `from`: in which CTA, and in how many
+        const int tiles = row_tiles(c, a, item / lay.subs);
+        const long long from = warp ? part_from[after_warp] : cta0 - start[0].y % tiles;
+        const int first_cta = run_of(from, per_cta), n = run_of(from + tiles - 1, per_cta) - first_cta + 1;
+        // its flags: that of part 2 first_cta + 1, then of every second one
+        u64* flags = reinterpret_cast<u64*>(static_cast<uint8_t*>(a.work) + kFlagsOffset) + 2 * first_cta + 1;
+        last = all_parts(flags, call, (int)blockIdx.x - first_cta, n);
+        if (lane == 0) join[warp] = make_int2(first_cta, n);
+      }
+      if (lane == 0 && !last) join[warp] = make_int2(0, 0);
     }
     __syncthreads();
-    if (!is_last || warp >= lay.count(it_sub)) continue;
+  }
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int item = which ? open_item[1] : open_item[0];
+    if (item < 0) continue;
+    const int it_row = item / lay.subs, it_sub = item - it_row * lay.subs, first_cta = join[which].x, n = join[which].y;
+    if (n == 0 || warp >= lay.count(it_sub)) continue;
+    __syncwarp();  // the factors of another item
     // a factor per part, in the ring's place; a batch of parts is loaded at once, the first beside the maxima
     const float* parts = static_cast<const float*>(a.work) + (size_t)2 * first_cta * kPartFloats;
     auto part = [&](int i) { return parts + (size_t)(2 * i + (i == 0)) * kPartFloats; };
