@@ -120,6 +120,23 @@ def test_min_p(min_p):
     check(x, "f32", 2, temperature=[0.9, 1.0, 1.1], min_p=[min_p] * 3)
 
 
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 1.3])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_min_p_at_weights_of_its_own_size(dtype, temperature):
+    """Logits in steps of 1/64 of the temperature, min_p the weight of one of them rounded to fp32: whether it reaches is
+    decided in the last bits, and the weights lie on the borders of a coarse view."""
+    import torch
+
+    t = np.float32(temperature)
+    steps = (3, 64, 100, 128, 192, 321)
+    for k in steps:
+        x = torch.tensor(np.float32(8.0) - (np.arange(400) / 64 * t).astype(np.float32))[torch.randperm(400, generator=torch.Generator().manual_seed(k))]
+        x = x[None].to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype])
+        # the weight of a token that is there, as the definition has it, rounded once
+        z = (x.double().max() - x.double().sort(descending=True).values[0, k]) / float(t)
+        check(x, dtype, k, temperature=[float(t)], min_p=[float(np.float32(np.exp(-float(z))))])
+
+
 def test_all_filters_with_rows_of_their_own():
     x = gaussian(24, 151936, "bf16", 8)
     r = np.random.RandomState(1)
@@ -176,6 +193,23 @@ def test_row_counts_that_share_the_gpu_differently(rows):
     js = [i * 7 % 600 for i in range(rows)]
     got, _ = run(x[::2], [(j + 0.5) / 12000 for j in js][: len(x[::2])], top_k=[12000] * len(x[::2]))
     assert list(got) == js[: len(got)]
+
+
+@pytest.mark.parametrize("rows", [1, 40, 150])
+def test_the_largest_vocabulary_with_one_value(rows):
+    """262143 tokens of one value just below the best: the sums at their largest, on 8, 4 and 1 CTAs per row."""
+    import torch
+
+    x = torch.zeros(rows, 262144)
+    x[:, 200000] = 0.0156
+    _, w = km.kept(x[0].numpy())
+    p = w / w.sum()
+    places = [0, 1, 2, 100000, 262142, 262143]
+    us = [float(np.cumsum(p)[at] - p[at] / 2) for at in places]
+    ids = [200000] + [i for i in range(262144) if i != 200000]
+    got, prob = run(x, [us[i % 6] for i in range(rows)])
+    assert list(got) == [ids[places[i % 6]] for i in range(rows)]
+    np.testing.assert_allclose(prob, [p[places[i % 6]] for i in range(rows)], rtol=2.0**-18)
 
 
 @pytest.mark.parametrize("spread", [1e-6, 1e-3, 0.05])

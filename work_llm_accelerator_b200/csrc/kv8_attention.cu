@@ -38,7 +38,7 @@ constexpr int kCtas = 148;  // one per SM; any number gives the same sums up to 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;    // tokens
-constexpr int kStages = 3;   // 8 KB each: 128 KB in flight per SM, three times what the latency asks for
+constexpr int kStages = 3;   // 8 KB each: two tiles of every warp under way, 128 KB per SM
 constexpr int kRows = 8;     // query heads of an item
 constexpr int kMinRun = 16;  // tiles of a CTA's run, at least: two for each warp
 constexpr int kSlack = 24;   // tiles by which a run may be longer to keep an item whole (about what a join costs)
@@ -99,7 +99,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// d = a b + c on int8 codes. `first`: c is the bits of kZero in every place.
+// d = a b + d on int8 codes; mma_first: d = a b + the bits of kZero.
 __device__ __forceinline__ void mma(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"

@@ -456,7 +456,8 @@ struct Row {
 #pragma unroll
       for (int i = 0; i < (int)(sizeof(e) / sizeof(float)); ++i) {
         const float v = seen(e[i]);
-        if (scale.bucket(v) == cmd.first && reaches_least(v)) atomicAdd(counted, 1);
+        const int b = scale.bucket(v);
+        if (b >= cmd.first && b <= cmd.last && reaches_least(v)) atomicAdd(counted, 1);
       }
     });
   }
@@ -678,11 +679,16 @@ struct Row {
     const Running& row = sh.row;
     const unsigned all = row.count[kBuckets - 1];
     if (k < 0 || (unsigned)k >= all) k = 0;
-    int least_bucket = kBuckets;
+    // Where min_p's border lies: tokens of these buckets are compared in 64 bits. A logit's own step count is rounded to
+    // fp32, so next to a bucket's border the neighbour is looked at too.
+    int least_from = kBuckets, least_to = kBuckets;
     if (use_least) {
       const double z = -log((double)least) * 64.0;
       use_least = z < kBuckets;
-      if (use_least) least_bucket = max(0, (int)z);
+      if (use_least) {
+        least_from = max(0, (int)(z - 1.0 / 512.0));
+        least_to = min(kBuckets - 1, max(0, (int)(z + 1.0 / 512.0)));
+      }
     }
     const double draw = u > 0.0f ? (double)u : 0.0;
 
@@ -715,10 +721,10 @@ struct Row {
       high = row.mass[to];
       cut_to = to;
     }
-    if (use_least && least_bucket <= cut_to) {
-      if (row.count[least_bucket] > row.before(least_bucket)) want_range(least_bucket, least_bucket);
-      low = min(low, row.mass_before(least_bucket));
-      high = row.mass[least_bucket];
+    if (use_least && least_from <= cut_to) {
+      if (row.count[least_to] > row.before(least_from)) want_range(least_from, least_to);
+      low = fmin(low, row.mass_before(least_from));
+      high = fmin(high, row.mass[least_to]);
     }
     want_range(row.find_mass(draw * low, true), min(cut_to, row.find_mass(draw * high, true)));
     int n_list = 0;
@@ -739,22 +745,23 @@ struct Row {
       const int b = row.find_mass(want, false);
       if (b < cut.bucket || (b == cut.bucket && cut.count > 0)) cut = resolve(b, 0, want, false, b < cut.bucket ? ~0u : cut.count, n_list, order);
     }
-    if (use_least && least_bucket <= cut.bucket) {
-      const unsigned has = row.count[least_bucket] - row.before(least_bucket);
+    if (use_least && least_from <= cut.bucket) {
+      const unsigned has = row.count[least_to] - row.before(least_from);
       unsigned in = 0;
       if (n_list) {
         if (has) {
-          const int from = first_of(n_list, [&](int i) { return scale.bucket(value_of(sh.list[i])) >= least_bucket; });
+          const int from = first_of(n_list, [&](int i) { return scale.bucket(value_of(sh.list[i])) >= least_from; });
           in = first_of((int)has + 1, [&](int i) { return i == (int)has || !reaches_least(value_of(sh.list[from + i])); });
         }
       } else {
-        ask({kCountLeast, least_bucket, least_bucket, 0, 0, 0, {}, {}});
+        ask({kCountLeast, least_from, least_to, 0, 0, 0, {}, {}});
         in = (unsigned)sh.counted;
       }
-      if (least_bucket < cut.bucket || in < cut.count) {
-        if (in == 0) cut = {least_bucket, 0, row.mass_before(least_bucket)};
-        else if (in == has) cut = {least_bucket, in, row.mass[least_bucket]};
-        else cut = resolve(least_bucket, in, 0.0, false, ~0u, n_list, order);
+      const unsigned reach = row.before(least_from) + in;  // at least 1: the best one
+      if (cut.bucket == kBuckets || reach < row.before(cut.bucket) + cut.count) {
+        const int b = row.find_count(reach);
+        if (row.count[b] == reach) cut = {b, reach - row.before(b), row.mass[b]};
+        else cut = resolve(b, reach - row.before(b), 0.0, false, ~0u, n_list, order);
       }
     }
     total = cut.mass;
