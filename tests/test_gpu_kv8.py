@@ -207,6 +207,28 @@ def test_read_equals_model(dtype, starts, counts):
         assert (out[w][off[-1] :] == 7.0).all()  # rows behind the last: as they were
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_read_into_wider_rows_and_nothing_to_read(dtype):
+    """Rows that lie inside wider ones: what is beside them stays; segments without a token write nothing."""
+    import torch
+    from work_llm_accelerator_b200 import host
+
+    c = Cache([90, 70], 2, seed=4)
+    for counts in ([33, 70], [0, 0]):
+        wide = torch.full((110, 7, km.HEAD), 7.0, dtype=dt(dtype)).cuda()
+        k, v = wide[:, 1:3], wide[:, 4:6]
+        a = [ints([1, 0]), ints([20, 5]), ints([0, counts[0], sum(counts)])]
+        host.kv8_read(c.handle, k.data_ptr(), v.data_ptr(), TYPES[dtype], wide.stride(0), 110, *(x.data_ptr() for x in a), 2,
+                      torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        want = torch.full((110, 7, km.HEAD), 7.0, dtype=dt(dtype))
+        for at, w in ((1, "k"), (4, "v")):
+            rows_ = np.concatenate([c.model[w].values(1, counts[0], 20), c.model[w].values(0, counts[1], 5)])
+            want[: sum(counts), at : at + 2] = torch.as_tensor(rows_).to(dt(dtype))
+        torch.testing.assert_close(wide.cpu(), want, rtol=0, atol=0, equal_nan=True)
+    assert host.kernel_error() == 0
+
+
 def test_more_segments_than_threads():
     """600 sequences of a token each, some of them empty: the segment search takes several passes."""
     r = np.random.RandomState(1)
@@ -502,6 +524,41 @@ def test_attention_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert torch.equal(outs[i], alone[i])
+
+
+def test_calls_on_a_stream_of_their_own_follow_it():
+    """Append, attention, read and sampling enqueued on a side stream behind work that is still running there."""
+    import torch
+    from work_llm_accelerator_b200 import host
+
+    c = filled([200], 2, seed=81)
+    r = np.random.RandomState(3)
+    x = rows(r, 8, 2)
+    side = torch.cuda.Stream()
+    src = {w: torch.as_tensor(x[w]).cuda() for w in "kv"}
+    late = {w: torch.zeros_like(src[w]) for w in "kv"}
+    a = [ints([0]), ints([150]), ints([0, 8])]
+    q = torch.randn(1, 12, 128, generator=torch.Generator().manual_seed(4)).cuda()
+    seqs, ns = ints([0]), ints([158])
+    out, lse = torch.zeros_like(q), torch.zeros(1, 12, device="cuda")
+    work = torch.empty(host.kv8_attention_workspace(1, 12, 2), dtype=torch.uint8, device="cuda")
+    back = {w: torch.zeros_like(src[w]) for w in "kv"}
+    busy = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            busy = busy @ busy * 1e-3
+        for w in "kv":
+            late[w].copy_(src[w])  # not there yet when the calls below are made
+        s = side.cuda_stream
+        host.kv8_append(c.handle, late["k"].data_ptr(), late["v"].data_ptr(), host.F32, 256, 8, *(v.data_ptr() for v in a), 1, s)
+        attend(c, q, "f32", seqs, ns, out=out, lse=lse, stream=side, work=work)
+        host.kv8_read(c.handle, back["k"].data_ptr(), back["v"].data_ptr(), host.F32, 256, 8, *(v.data_ptr() for v in a), 1, s)
+    torch.cuda.synchronize()
+    for w in "kv":
+        c.model[w].append(x[w], 0, 150)
+        np.testing.assert_array_equal(back[w].cpu().numpy(), c.model[w].values(0, 8, 150))
+    check_rows(c, q, "f32", [0], [158], out, lse)
 
 
 def test_attention_block_offsets_past_31_bits():
