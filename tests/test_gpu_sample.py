@@ -345,3 +345,28 @@ def test_engine_samples_from_its_own_logits():
             eng.sample([0.5] * 3)  # kept no logits
     finally:
         eng.close()
+
+
+@pytest.mark.parametrize("rows", [1, 18, 19, 74, 75, 148])
+@pytest.mark.parametrize("vocab", [8193, 20000])
+def test_short_rows_on_several_ctas_started_one_by_one(rows, vocab):
+    """A row's CTAs exchange their largest logits after a first pass of a microsecond. Launches behind work that frees its
+    SMs one at a time start them apart: every row still has the argmax of all its parts."""
+    import torch
+    from work_llm_accelerator_b200 import host
+
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, vocab, generator=g).cuda()
+    want = x.argmax(1).to(torch.int32)
+    zero, t = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    tokens = torch.full((40, rows), -9, dtype=torch.int32, device="cuda")
+    other = torch.cuda.Stream()
+    busy = torch.randn(3000, 700, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(40):
+        with torch.cuda.stream(other):
+            busy = (busy * 1.0001).sin()
+        host.sample(x.data_ptr(), host.F32, rows, vocab, vocab, t.data_ptr(), 0, 0, 0, zero.data_ptr(), tokens[i].data_ptr(), 0,
+                    torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert (tokens == want[None]).all()

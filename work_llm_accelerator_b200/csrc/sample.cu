@@ -787,6 +787,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kCl == k
   Shared& sh = *reinterpret_cast<Shared*>(smem);
   const int row = blockIdx.x / kCl, rank = blockIdx.x % kCl, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   R r(sh);
+  // another CTA's shared memory may be written once that CTA has started: each says so here, and waits below
+  if (kCl > 1) cg::this_cluster().barrier_arrive();
   r.lo = min(a.vocab, rank * slice);
   r.n = min(slice, a.vocab - r.lo);
   r.x = static_cast<const typename R::T*>(a.logits) + (long long)row * a.stride + r.lo;
@@ -809,6 +811,7 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kCl == k
   for (int s = 16; s > 0; s >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, s));
   if (lane == 0) sh.warp_best[warp] = best;
   __syncthreads();
+  if (kCl > 1) cg::this_cluster().barrier_wait();
   if (threadIdx.x < kCl) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) best = max(best, sh.warp_best[w]);
