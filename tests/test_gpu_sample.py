@@ -370,3 +370,44 @@ def test_short_rows_on_several_ctas_started_one_by_one(rows, vocab):
                     torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     assert (tokens == want[None]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 18, 40, 75, 150])
+@pytest.mark.parametrize("u", [1.0, 7.0, 3e38, float("inf")])
+def test_uniform_numbers_from_one_on_take_the_last_kept_token(rows, u):
+    """Thousands of ties around the border of what is kept and thousands of tokens behind it, none of which may be counted
+    with the draw: [0, 1) is asked for, but the numbers lie on the device, where nothing else checks them."""
+    import torch
+
+    x = torch.full((rows, 60000), -9.0)
+    r = np.random.RandomState(rows)
+    places = r.permutation(60000)
+    x[:, np.sort(places[:20000])] = 1.0
+    x[:, np.sort(places[20000:39000])] = 0.5
+    x[:, places[39000]] = -3.0
+    one = np.sort(places[:20000])
+    second = np.sort(places[20000:39000])
+    rest = np.setdiff1d(np.arange(60000), places[:39001])
+    got, p = run(x, [u] * rows, top_k=[10000] * rows)
+    assert (got == one[9999]).all()
+    np.testing.assert_allclose(p, 1e-4, rtol=2.0**-18)
+    got, _ = run(x, [u] * rows, top_k=[20000] * rows)  # the border is the bucket's
+    assert (got == one[19999]).all()
+    got, _ = run(x, [u] * rows, top_k=[25000] * rows)
+    assert (got == second[4999]).all()
+    # half of the first 20000: top_p in the middle of a share
+    got, _ = run(x, [u] * rows, top_k=[20000] * rows, top_p=[(9999 + 0.5) / 20000] * rows)
+    assert (got == one[9999]).all()
+    got, _ = run(x, [u] * rows, min_p=[0.5] * rows)  # exp(-1 / 2) = 0.607, exp(-4) = 0.018
+    assert (got == second[-1]).all()
+    got, _ = run(x, [u] * rows, min_p=[0.01] * rows)
+    assert (got == places[39000]).all()
+    got, _ = run(x, [u] * rows)
+    assert (got == rest[-1]).all()
+    # few tokens in every bucket, all filters: what is listed and sorted at once
+    x = gaussian(rows, 20000, "f32", rows)
+    k, t = [50] * rows, [0.9] * rows
+    top_p = safe_top_p(x, t, k, 0.9)
+    got, _ = run(x, [u] * rows, temperature=t, top_k=k, top_p=top_p)
+    want = [km.kept(x[i].numpy(), float(np.float32(0.9)), 50, float(np.float32(top_p[i])))[0][-1] for i in range(rows)]
+    np.testing.assert_array_equal(got, want)

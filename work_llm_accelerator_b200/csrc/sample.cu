@@ -690,7 +690,7 @@ struct Row {
         least_to = min(kBuckets - 1, max(0, (int)(z + 1.0 / 512.0)));
       }
     }
-    const double draw = u > 0.0f ? (double)u : 0.0;
+    const double draw = u > 0.0f ? fmin((double)u, 1.0) : 0.0;  // from 1 on: the last one kept
 
     // The buckets that borders and draw may fall in, from the sums alone: a border inside a bucket leaves the mass up to
     // it between that before and that behind the bucket, and so what depends on it between two buckets. Mostly they
@@ -699,6 +699,7 @@ struct Row {
     Command cmd{kGather, kBuckets, 0, 0, 0, 0, {}, {}};
     unsigned listed = 0;
     auto want_range = [&](int from, int to) {
+      from = min(from, to);  // a draw of all that is kept is sought behind it
       cmd.from[cmd.ranges] = from;
       cmd.to[cmd.ranges++] = to;
       cmd.first = min(cmd.first, from);
@@ -730,7 +731,7 @@ struct Row {
     int n_list = 0;
     if (listed <= kList) {
       ask(cmd);
-      n_list = sh.listed;
+      n_list = sh.listed <= kList ? sh.listed : 0;  // the list's bounds do not rest on the sums
       sort_list(n_list);
     }
 
