@@ -411,3 +411,40 @@ def test_uniform_numbers_from_one_on_take_the_last_kept_token(rows, u):
     got, _ = run(x, [u] * rows, temperature=t, top_k=k, top_p=top_p)
     want = [km.kept(x[i].numpy(), float(np.float32(0.9)), 50, float(np.float32(top_p[i])))[0][-1] for i in range(rows)]
     np.testing.assert_array_equal(got, want)
+
+
+def step_borders(dtype, n):
+    """(temperature, distance) pairs, fp32 and of the type: 64 * distance / temperature lies below a whole number but rounds
+    to it in fp32."""
+    r = np.random.RandomState(7)
+    found = []
+    while len(found) < n:
+        t = (0.5 + r.rand(1000)).astype(np.float32)
+        c = np.float32(64) * (np.float32(1) / t)
+        bits = {"f32": 24, "f16": 11, "bf16": 8}[dtype]
+        d = np.ldexp(r.randint(1 << (bits - 1), 1 << bits, 1000), 2 - bits).astype(np.float32)  # 2 to 4
+        exact = c[:, None].astype(np.float64) * d[None, :]  # 48 bits at most
+        near = exact.astype(np.float32)
+        i, j = np.nonzero((near == np.rint(near)) & (near > exact) & (near >= 128) & (near < 256))
+        found = list(dict.fromkeys(found + [(float(t[a]), float(d[b])) for a, b in zip(i, j)]))
+    return found[:n]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [6, 24, 78, 156])
+def test_logits_that_round_to_a_border(dtype, rows):
+    """Distances whose steps round up to a border between two coarse views, thousands of tokens at each: the sums and the
+    search for a token must put them on the same side. On 8, 4, 2 CTAs per row and one, in every type."""
+    import torch
+
+    pairs = step_borders(dtype, 6)
+    x = torch.full((rows, 9000), float("-inf"))
+    for i in range(rows):
+        many = [3000, 300][i % 2]
+        places = np.random.RandomState(i).permutation(9000)
+        x[i, places[0]] = 0.0
+        x[i, places[1 : 1 + many]] = -pairs[i % 6][1]
+    x = x.to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype])
+    t = [pairs[i % 6][0] for i in range(rows)]
+    check(x, dtype, rows, temperature=t)
+    check(x, dtype, rows + 1, temperature=t, top_k=[[1500, 150][i % 2] for i in range(rows)])

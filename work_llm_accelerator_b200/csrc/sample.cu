@@ -27,6 +27,7 @@
 
 #include <algorithm>
 
+#include "qwen_common.cuh"
 #include "sample.h"
 
 namespace cg = cooperative_groups;
@@ -99,31 +100,9 @@ __device__ __forceinline__ u64 order_of(float x, int i) { return (u64)key_of(x) 
 __device__ __forceinline__ int index_of(u64 order) { return kMaxVocab - 1 - (int)(order & (kMaxVocab - 1)); }
 __device__ __forceinline__ float value_of(u64 order) { return value_of((unsigned)(order >> 18)); }
 
-// Pairs of fp32 numbers in one instruction.
-typedef u64 F2;
-__device__ __forceinline__ F2 pair(float x, float y) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(F2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ F2 add2_down(F2 a, F2 b) {
   F2 r;
-  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
 
@@ -158,18 +137,21 @@ struct Scale {
     const float d = top - x, f = fmaf(d, c_low, fmaf(d, c, -b));
     return __float_as_uint(fmaf(f, fmaf(f, fmaf(f, fmaf(f, k4, k3), k2), k1), kRound));
   }
-  // The same for two logits: bucket (in the low bits of `up`) and q.
-  __device__ __forceinline__ void two(float x, float y, float2& steps, float2& up, float2& q) const {
-    const F2 minus = pair(-1.0f, -1.0f), tops = pair(top, top), cs = pair(c, c);
-    const F2 d = fma2(pair(x, y), minus, tops), t = mul2(d, cs), u = add2_down(t, pair(kFloor, kFloor));
-    F2 f = fma2(u, minus, pair(kFloor, kFloor));  // - floor
-    f = fma2(d, pair(c_low, c_low), fma2(d, cs, f));
-    F2 e = fma2(f, pair(k4, k4), pair(k3, k3));
-    e = fma2(f, e, pair(k2, k2));
-    e = fma2(f, e, pair(k1, k1));
-    q = unpair(fma2(f, e, pair(kRound, kRound)));
-    steps = unpair(t);
-    up = unpair(u);
+  // The same for two logits: bucket (in the low bits of `up`) and q. The steps are rounded before the floor is taken, as
+  // `bucket` does it: a product that ran into the addition would put some logits into another bucket than the one they
+  // are listed from. nz = f2_negzero() keeps it apart.
+  __device__ __forceinline__ void two(float x, float y, F2 nz, float2& steps, float2& up, float2& q) const {
+    const F2 minus = f2(-1.0f, -1.0f), tops = f2(top, top), cs = f2(c, c);
+    const F2 d = fma2(f2(x, y), minus, tops), t = mul2(d, cs, nz), u = add2_down(t, f2(kFloor, kFloor));
+    F2 f = fma2(u, minus, f2(kFloor, kFloor));  // - floor
+    f = fma2(d, f2(c_low, c_low), fma2(d, cs, f));
+    F2 e = fma2(f, f2(k4, k4), f2(k3, k3));
+    e = fma2(f, e, f2(k2, k2));
+    e = fma2(f, e, f2(k1, k1));
+    e = fma2(f, e, f2(kRound, kRound));
+    q = make_float2(f2_lo(e), f2_hi(e));
+    steps = make_float2(f2_lo(t), f2_hi(t));
+    up = make_float2(f2_lo(u), f2_hi(u));
   }
   // the weight in 64 bits, as the sums have it
   __device__ double weight(float x) const {
@@ -333,6 +315,7 @@ struct Row {
     u64 q[kPerThread] = {};
     const int shift = kOrderBits - cmd.bits, digit = min(kDigit, shift);
     const int first = threadIdx.x * kPerThread;
+    const F2 nz = f2_negzero();
     const unsigned hist = (unsigned)__cvta_generic_to_shared(&sh.hist[0][0]) - 4 * __float_as_uint(Scale::kFloor);
     for (int from = 0; from < max(n, 1); from += kFold) {
       clear_histogram();
@@ -363,7 +346,7 @@ struct Row {
 #pragma unroll
           for (int i = 0; i + 1 < kN; i += 2) {
             float2 t, up, q;
-            scale.two(v[i], v[i + 1], t, up, q);
+            scale.two(v[i], v[i + 1], nz, t, up, q);
             // 4 * (bits of up) is 4 * bucket and a constant that goes into the address
             const unsigned a0 = hist + 4 * __float_as_uint(up.x), a1 = hist + 4 * __float_as_uint(up.y);
             if (Scale::counts(t.x)) count_one(a0, __float_as_uint(q.x));
