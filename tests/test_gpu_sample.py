@@ -448,3 +448,40 @@ def test_logits_that_round_to_a_border(dtype, rows):
     t = [pairs[i % 6][0] for i in range(rows)]
     check(x, dtype, rows, temperature=t)
     check(x, dtype, rows + 1, temperature=t, top_k=[[1500, 150][i % 2] for i in range(rows)])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [16, 64, 148, 200])
+def test_numbers_on_the_borders_between_tokens(dtype, rows):
+    """A uniform number and a top_p that round to the sum at a token's end, with wide gaps between the logits: either
+    neighbour may be drawn (the sums are those of other roundings), never a token that is not there."""
+    import torch
+
+    r = np.random.RandomState(rows)
+    vocab = 9000
+    x = torch.full((rows, vocab), float("-inf"))
+    for i in range(rows):
+        n = [40, 3000][i % 2]  # every second row: levels of a hundred ties each, more than are sorted at once
+        level = np.sort(r.randint(0, 600, 30))[r.randint(0, 30, n)] / 40.0
+        x[i, r.permutation(vocab)[:n]] = torch.as_tensor(-level, dtype=torch.float32)
+    x = x.to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype])
+    for turn in range(8):
+        us, near, ps = [], [], []
+        for i in range(rows):
+            ids, w = km.kept(x[i].float().numpy(), 0.7)
+            p = np.cumsum(w) / w.sum()
+            # ends of levels, where the next weight may be buckets away
+            last = np.nonzero(np.append(np.diff(w) < 0, False))[0]
+            at = int(r.choice(last[w[last] / w.sum() > 1e-5]))
+            if turn % 2:  # top_p at the border, the draw at its end: the last token that top_p keeps
+                ps.append(float(np.float32(p[at])))
+                us.append(1.0)
+            else:
+                ps.append(1.0)
+                us.append(float(np.float32(p[at])))
+            # within 2^-19 of the whole, all that the weights' roundings and that of the number can move
+            lo, hi = np.searchsorted(p, [p[at] - 2.0**-19, p[at] + 2.0**-19])
+            near.append({int(v) for v in ids[lo : hi + 1]})
+        got, _ = run(x, us, dtype, temperature=[float(np.float32(0.7))] * rows, top_p=ps if turn % 2 else None)
+        for i in range(rows):
+            assert int(got[i]) in near[i], (turn, i, int(got[i]))

@@ -203,7 +203,10 @@ struct Running {
   }
   __device__ int find_mass(double want, bool more) const {
     const int b = first_of(kBuckets, [&](int i) { return more ? mass[i] > want : mass[i] >= want; });
-    return b < kBuckets - 1 ? b : find_count(count[kBuckets - 1]);
+    if (count[b] > before(b)) return b;
+    // none does, or one without tokens: threads add up the running sums in orders of their own, so that they may rise by a
+    // rounding there. The next one with tokens.
+    return find_count(min(before(b) + 1, count[kBuckets - 1]));
   }
   __device__ unsigned before(int b) const { return b ? count[b - 1] : 0; }
   __device__ double mass_before(int b) const { return b ? mass[b - 1] : 0.0; }
@@ -609,11 +612,13 @@ struct Row {
   // A mass inside bucket b, kept from leaving it by the rounding of its sum.
   __device__ double within(int b, double m) const { return fmin(fmax(m, sh.row.mass_before(b)), sh.row.mass[b]); }
   // Inside bucket b: the cut at the first token with at least `need` tokens of the bucket up to it (need > 0), or a mass
-  // of everything up to it that reaches (more: exceeds) want; at most `most` tokens. Also that token. `listed`: the
-  // sorted list holds all of the bucket, among others.
-  __device__ Cut resolve(int b, unsigned need, double want, bool more, unsigned most, int listed, u64& order) {
+  // of everything up to it that reaches (more: exceeds) want; at most `most` tokens. Also that token. `listed`: the length
+  // of the sorted list, which holds whole buckets; 0 as soon as a bucket had to be gathered by itself.
+  __device__ Cut resolve(int b, unsigned need, double want, bool more, unsigned most, int& listed, u64& order) {
+    const int from = first_of(listed, [&](int i) { return scale.bucket(value_of(sh.list[i])) >= b; });
+    // a rounding may have moved a border into a bucket that is not in the list
+    if (listed && scale.bucket(value_of(sh.list[from])) != b) listed = 0;
     if (listed) {
-      const int from = first_of(listed, [&](int i) { return scale.bucket(value_of(sh.list[i])) >= b; });
       const unsigned n_in = sh.row.count[b] - sh.row.before(b);
       const double m0 = sh.row.mass_before(b) - (from ? sh.prefix[from - 1] : 0.0);
       const int at = first_of((int)min(min(most, n_in), (unsigned)(listed - from)), [&](int i) {
@@ -756,8 +761,7 @@ struct Row {
     } else {  // the draw fell behind the cut by a rounding: the last one kept
       const unsigned kept = row.before(cut.bucket) + cut.count;
       b = row.find_count(kept);
-      // its bucket need not be among those that are listed
-      resolve(b, kept - row.before(b), 0.0, false, ~0u, 0, order);
+      resolve(b, kept - row.before(b), 0.0, false, ~0u, n_list, order);
     }
   }
 };
