@@ -95,7 +95,8 @@ int qwen_engine_read_trace(qwen_engine* e, unsigned long long* out, long long n,
 int qwen_engine_read_logits(qwen_engine* e, float* out, long long n_floats);
 /* Sample one token for each of the n rows of the last prefill / decode call instead of taking its argmax: the logits
  * stay on the device (option "logits" must have been on during that call; n must be its rows -- with more than 4
- * sequences that are not one batched step, those of its last group of 4). Settings per row, each array may be NULL:
+ * sequences that are not one batched step, those of its last group of 4). Where that call failed, or a bench or profile
+ * call ran steps after it, there is nothing to sample from and the call is refused. Settings per row, each array may be NULL:
  * temperature (1), top_k, top_p, min_p (off), as in qwen_b200_sample (qwen_b200_ops.h); uniforms [n] in [0, 1).
  * tokens [n] and probs [n] (or NULL) receive the tokens and their probabilities among the kept ones. Host buffers; the
  * call returns after the results are on the host. Feed the tokens to the next qwen_engine_decode. */

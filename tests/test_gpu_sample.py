@@ -485,3 +485,41 @@ def test_numbers_on_the_borders_between_tokens(dtype, rows):
         got, _ = run(x, us, dtype, temperature=[float(np.float32(0.7))] * rows, top_p=ps if turn % 2 else None)
         for i in range(rows):
             assert int(got[i]) in near[i], (turn, i, int(got[i]))
+
+
+def test_engine_keeps_no_logits_of_steps_that_were_not_asked_for():
+    """After profiled or timed steps, or a call that failed on its way, there is nothing to sample from."""
+    from work_llm_accelerator_b200 import host
+
+    eng = host.Engine(0, 8, max_seqs=8, max_len=256)
+    try:
+        eng.init_synthetic(5)
+        eng.set_option("logits", 1)
+        for slot in range(8):
+            eng.prefill(slot, [slot + 1, 7])
+
+        def dropped(call, n, slots):
+            eng.decode(slots, [3] * n)
+            eng.sample([0.5] * n)
+            call()
+            with pytest.raises(host.EngineError, match="logits"):
+                eng.sample([0.5] * n)
+
+        def fails(call):
+            with pytest.raises(host.EngineError):
+                call()
+
+        dropped(lambda: eng.profile_decode(0, 9, 2), 1, [0])
+        dropped(lambda: eng.bench_decode([0], [9], 2, 1), 1, [0])
+        dropped(lambda: eng.profile_batched(range(8), [9] * 8, 2), 8, range(8))
+        dropped(lambda: fails(lambda: eng.decode([0, 99], [3, 3])), 2, [0, 1])
+        dropped(lambda: fails(lambda: eng.prefill_chunk(0, [5] * 255)), 1, [0])
+        dropped(lambda: fails(lambda: eng.prefill(0, [5])), 1, [0])  # the slot is not empty
+        eng.set_option("batched", 0)
+        # two groups, the second of which is refused after the first has run
+        dropped(lambda: fails(lambda: eng.decode([0, 1, 2, 3, 99, 5, 6, 7], [3] * 8)), 4, [0, 1, 2, 3])
+        eng.decode(range(6), [3] * 6)
+        eng.sample([0.5, 0.5])  # the last group
+        assert list(eng.sample([0.5, 0.5], temperature=[0.0, 0.0])[0]) == list(eng.read_logits(2).argmax(1))
+    finally:
+        eng.close()

@@ -191,7 +191,7 @@ struct qwen_engine {
   float* dump = nullptr;
   float* logits = nullptr;
   int last_rows = 0;
-  int logits_rows = 0;           // rows of `logits` that the last call wrote, 0 if it kept none
+  int logits_rows = 0;           // rows of `logits` that the last prefill / decode call left, 0 if it kept none or failed
   float* sample_io = nullptr;    // settings and results of qwen_engine_sample, 7 words a row
   int sample_cap = 0;
   // rope tables
@@ -1139,6 +1139,11 @@ int qwen_engine_set_option(qwen_engine* e, const char* name, long long value) {
 
 namespace {
 
+// At the beginning of every call that runs an LM head, refused ones included; note_rows at the end of a prefill / decode
+// call that kept its logits.
+void drop_logits(qwen_engine* e) {
+  if (e) e->logits_rows = 0;
+}
 void note_rows(qwen_engine* e, int n) {
   e->last_rows = n;
   e->logits_rows = e->keep_logits || e->exact ? n : 0;
@@ -1174,6 +1179,7 @@ int prefill_at(qwen_engine* e, int slot, const int32_t* tokens, int n, int past,
 }  // namespace
 
 int qwen_engine_prefill(qwen_engine* e, int slot, const int32_t* tokens, int n, int32_t* next_token) {
+  drop_logits(e);
   if (!e || slot < 0 || slot >= e->max_seqs || !tokens || n <= 0 || n > e->max_len) return kStatusInvalid;
   if (e->seq_len[slot] != 0) {
     set_error("prefill into a non-empty slot %d (reset it first, or continue it with qwen_engine_prefill_chunk)",
@@ -1184,11 +1190,13 @@ int qwen_engine_prefill(qwen_engine* e, int slot, const int32_t* tokens, int n, 
 }
 
 int qwen_engine_prefill_chunk(qwen_engine* e, int slot, const int32_t* tokens, int n, int32_t* next_token) {
+  drop_logits(e);
   if (!e || slot < 0 || slot >= e->max_seqs || !tokens || n <= 0) return kStatusInvalid;
   return prefill_at(e, slot, tokens, n, e->seq_len[slot], next_token);
 }
 
 int qwen_engine_decode(qwen_engine* e, const int32_t* slots, const int32_t* tokens, int n, int32_t* next_tokens) {
+  drop_logits(e);
   if (!e || !slots || !tokens || n <= 0) return kStatusInvalid;
   E_TRY(cudaSetDevice(e->device));
   if (batched_ok(e, n)) {
@@ -1248,17 +1256,18 @@ int qwen_engine_decode(qwen_engine* e, const int32_t* slots, const int32_t* toke
       next_tokens[base + i] = e->h_io[12 + i];
       e->seq_len[slots[base + i]] += 1;
     }
-    note_rows(e, nt);
+    e->last_rows = nt;
   }
+  note_rows(e, e->last_rows);
   return 0;
 }
 
 int qwen_engine_bench_decode(qwen_engine* e, const int32_t* slots, const int32_t* first_tokens, int n, int steps,
                              int warmup, float* ms_per_step) {
+  drop_logits(e);
   if (!e || !slots || !first_tokens || n <= 0 || steps <= 0 || warmup < 0) return kStatusInvalid;
   if (n > kGemvMaxTokens && !batched_ok(e, n)) return kStatusInvalid;
   E_TRY(cudaSetDevice(e->device));
-  e->logits_rows = 0;
   if (n > kGemvMaxTokens) {
     int max_end = 0;
     for (int i = 0; i < n; ++i) {
@@ -1334,6 +1343,7 @@ int qwen_engine_bench_decode(qwen_engine* e, const int32_t* slots, const int32_t
 }
 
 int qwen_engine_profile_decode(qwen_engine* e, int slot, int first_token, int steps, float* ms_out) {
+  drop_logits(e);
   if (!e || slot < 0 || slot >= e->max_seqs || steps <= 0 || !ms_out) return kStatusInvalid;
   E_TRY(cudaSetDevice(e->device));
   const int end = e->seq_len[slot] + steps;
@@ -1373,6 +1383,7 @@ int qwen_engine_profile_decode(qwen_engine* e, int slot, int first_token, int st
 
 int qwen_engine_profile_batched(qwen_engine* e, const int32_t* slots, const int32_t* first_tokens, int n, int steps,
                                 float* ms_out) {
+  drop_logits(e);
   if (!e || !slots || !first_tokens || !ms_out || steps <= 0 || !batched_ok(e, n)) return kStatusInvalid;
   E_TRY(cudaSetDevice(e->device));
   int max_end = 0;
@@ -1563,6 +1574,7 @@ int qwen_engine_sample(qwen_engine* e, int n, const float* temperature, const in
 
 int qwen_engine_decode_device(qwen_engine* e, const int32_t* slots, const int32_t* d_tokens, int n,
                               int32_t* d_next) {
+  drop_logits(e);
   if (!e || !slots || !d_tokens || !d_next || n <= 0) return kStatusInvalid;
   const bool batched = batched_ok(e, n);
   if (n > kGemvMaxTokens && !batched) return kStatusInvalid;
