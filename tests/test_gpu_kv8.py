@@ -655,3 +655,20 @@ def test_decode_loop_in_a_graph():
                 assert cum[j] - 1e-5 - w[-1] / w.sum() <= ui <= cum[j + 1] + 1e-5 + w[-1] / w.sum()
     c.check(lens)
     assert host.kernel_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_queries_near_the_largest_number(dtype):
+    """Queries on both sides of 2^127, up to the largest finite value of the type, with a scale that brings them back to 1."""
+    import torch
+
+    lens = [300, 64, 1]
+    c = filled(lens, 2, seed=22)
+    g = torch.Generator().manual_seed(6)
+    q = (2 * torch.rand(3, 12, 128, generator=g) - 1) * torch.tensor([3.3e38, 1.7e38, 2.5e38])[:, None, None]
+    q[0, 0, 0], q[1, 0, 0] = torch.finfo(dt(dtype)).max, 2.0**127
+    q = q.to(dt(dtype)).cuda()
+    assert torch.isfinite(q).all()
+    scale = 2.0**-128
+    out, lse, _ = attend(c, q, dtype, ints([0, 1, 2]), ints(lens), scale=scale)
+    check_rows(c, q, dtype, [0, 1, 2], lens, out, lse, scale=scale)

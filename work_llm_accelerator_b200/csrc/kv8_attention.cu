@@ -403,13 +403,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^21 and less of them, with the row's largest value in [2^21, 2^22) after the scaling; a NaN or an infinity in
       // the row makes all its scores NaN
-      const int e = top == 0 ? 127 : min(253, max(1, (int)(top >> 23)));
-      const float down = __uint_as_float((unsigned)(254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
+      const int e = top == 0 ? 127 : min(254, max(1, (int)(top >> 23)));
+      // the exponent of 2^-127 is none of a normal number: half of it goes into the unit
+      const float down = __uint_as_float((unsigned)max(1, 254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
+      const float unit = e == 254 ? 1048576.0f : 2097152.0f;
       q.scale = top >= 0x7f800000u ? __int_as_float(0x7fc00000) : a.scale * up * (1.4426950408889634f / 2097152.0f);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        by_digit(digits(fmaf(x[i].x * down, 2097152.0f, kZero)), digits(fmaf(x[i].y * down, 2097152.0f, kZero)),
-                 digits(fmaf(x[i].z * down, 2097152.0f, kZero)), digits(fmaf(x[i].w * down, 2097152.0f, kZero)), q.d[i]);
+        by_digit(digits(fmaf(x[i].x * down, unit, kZero)), digits(fmaf(x[i].y * down, unit, kZero)),
+                 digits(fmaf(x[i].z * down, unit, kZero)), digits(fmaf(x[i].w * down, unit, kZero)), q.d[i]);
     };
 
     int it_row = row, it_sub = sub;
