@@ -85,7 +85,8 @@ int qwen_b200_prefill_approx_exp(const float* x, float* y, long long n, void* st
  * x, y [n] fp32 device memory. */
 int qwen_b200_exact_expf(const float* x, float* y, long long n, void* stream);
 
-/* Element types of the operators below. Whatever the type, they compute in fp32 and round results once. */
+/* Element types of the operators below. Whatever the type, they compute in fp32 or, as said there, in integers of about as
+ * many bits, and round results once. */
 enum { QWEN_B200_F32 = 0, QWEN_B200_F16 = 1, QWEN_B200_BF16 = 2 };
 
 /* An 8-bit KV cache of one layer, in buffers of the caller (device memory): blocks of 64 tokens, head dimension
@@ -141,6 +142,9 @@ int qwen_b200_kv8_read(const qwen_b200_kv8_cache* cache, void* k, void* v, int d
  * row_seqs[r] attends to the sequence's first row_lens[r] tokens (its own included: append first); drafted tokens of
  * one sequence are rows with lengths that rise by one. Query head h reads kv head h / (n_q_heads / n_kv_heads).
  *   s_j = scale * (q . k_j),  out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j)
+ * Both products are sums of integers: a query head is held to 2^-30 of its largest channel, and a weight to 2^-30 of the
+ * largest of the up to 32 tokens that it is computed with, in place of 2^-24 of itself; the sums are exact, and what
+ * follows is fp32.
  * row_lens[r] == 0: out is 0 and lse -infinity. row_seqs[r] < 0 (a padded row): out and lse are left as they are.
  *   q, out     [n_rows] rows of n_q_heads x 128 values of `dtype` (16-byte aligned, strides in elements, multiples
  *              of 16 bytes); out must not overlap q

@@ -672,3 +672,75 @@ def test_attention_queries_near_the_largest_number(dtype):
     scale = 2.0**-128
     out, lse, _ = attend(c, q, dtype, ints([0, 1, 2]), ints(lens), scale=scale)
     check_rows(c, q, dtype, [0, 1, 2], lens, out, lse, scale=scale)
+
+
+def values64(c, w, seq, n):
+    """code * scale in 64 bits, where the model rounds it to fp32 as the reading back does (2^-24 of a value, which is more
+    than the bounds below leave)."""
+    pos = np.arange(n)
+    b = c.table[seq, pos // km.BLOCK]
+    return c.model[w].codes[b, :, pos % km.BLOCK] * c.model[w].scales[b].astype(np.float64)[:, :, None]
+
+
+def score_bound(q, k, scale, s):
+    """How far a score may be off: q is held to 2^-30 of its row's largest channel (half a step of 31-bit integers; the
+    2^-6 covers the digits' joining), the exact digit products are joined, scaled and carried to lse in at most 12
+    roundings of 2^-24."""
+    q, k = np.abs(np.asarray(q, np.float64)), np.abs(np.asarray(k, np.float64))
+    return abs(scale) * 2.0**-30 * (1 + 2.0**-6) * q.max(-1) * k.sum(-1) + 12 * 2.0**-24 * np.abs(s)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ratio,code", [(1.0, 1.0), (50.0, 1.0), (200.0, 0.02), (1000.0, 0.0), (30000.0, 0.0), (1000.0, 0.01)])
+def test_attention_one_large_channel(dtype, ratio, code):
+    """A channel far larger than the others, whose keys are small or zero: the others must not lose their bits to it. With one
+    token, lse is its score."""
+    import torch
+
+    n = 40
+    c = filled([1] * n, 2, seed=23)
+    for b in c.table[:, 0]:
+        c.model["k"].codes[b, :, 0, 17] = np.rint(code * c.model["k"].codes[b, :, 0, 17])
+    c.codes["k"].copy_(torch.as_tensor(c.model["k"].codes.astype(np.int8)))
+    q = torch.randn(n, 12, 128, generator=torch.Generator().manual_seed(int(ratio)))
+    q[:, :, 17] *= ratio / q[:, :, 17].abs()
+    q = q.to(dt(dtype)).cuda()
+    out, lse, _ = attend(c, q, dtype, ints(range(n)), ints([1] * n))
+    q, lse = q.float().cpu().numpy().astype(np.float64), lse.cpu().numpy()
+    for r in range(n):
+        k = values64(c, "k", r, 1)[0]
+        for h in range(12):
+            want = float(k[h // 6] @ q[r, h] * np.float32(SCALE))
+            assert abs(lse[r, h] - want) <= score_bound(q[r, h], k[h // 6], SCALE, want), (r, h, lse[r, h] - want)
+    check_rows(c, torch.as_tensor(q), dtype, list(range(n)), [1] * n, out, torch.as_tensor(lse))
+
+
+@pytest.mark.parametrize("below", [2.0, 5.0, 8.0, 11.0, 14.0])
+def test_attention_small_weights_beside_a_large_one(below):
+    """A first token that takes almost all of the weight and whose values are zero: the result is that of the others in its
+    tile. Their weights are held to 2^-30 of the largest."""
+    import torch
+
+    u, n = 2.0**-24, 32
+    c = filled([n], 1, seed=24)
+    b = c.table[0, 0]
+    for w in "kv":
+        c.model[w].codes[b, 0, 0] = 0.0
+        c.model[w].scales[b] = 0.01
+    c.model["k"].codes[b, 0, 1:] = np.rint(c.model["k"].codes[b, 0, 1:] / 16) - 100
+    for w in "kv":
+        c.codes[w].copy_(torch.as_tensor(c.model[w].codes.astype(np.int8)))
+        c.scales[w].copy_(torch.as_tensor(c.model[w].scales))
+    q = (below / (128 * SCALE) * (0.5 + torch.rand(1, 6, 128, generator=torch.Generator().manual_seed(3)))).cuda()
+    out, lse, _ = attend(c, q, "f32", ints([0]), ints([n]))
+    k, v = (values64(c, w, 0, n)[:, 0] for w in "kv")
+    got, qs = out[0].cpu().numpy(), q[0].cpu().numpy().astype(np.float64)
+    for h in range(6):
+        s = k @ qs[h] * np.float32(SCALE)
+        p = np.exp(s - s.max())
+        d = score_bound(qs[h], k, SCALE, s).max()
+        want = p @ v / p.sum()
+        # weights: 2^-30 each, 2 d from the scores, 4 u from the exponential; sums of 32 and the last steps: 48 u
+        tol = 2.0**-30 * (1 + 2.0**-6) * np.abs(v).sum(0) / p.sum() + (2 * d + 52 * u) * (p @ np.abs(v)) / p.sum() + 2.0**-149
+        assert (np.abs(got[h] - want) <= tol).all(), (h, np.abs(got[h] - want).max(), tol.min())
+        assert abs(float(lse[0, h]) - (s.max() + np.log(p.sum()))) <= 2 * d + 52 * u

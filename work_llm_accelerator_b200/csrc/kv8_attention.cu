@@ -4,17 +4,19 @@
 // Mathematics. With k_j = s_k c_j and v_j = s_v d_j (int8 codes, one scale per 64-token block) a score is
 // (scale s_k) (q . c_j), and a tile of 32 tokens adds s_v sum_j p_j d_j. Both sums run on the codes as they lie in the
 // cache, on the int8 tensor cores (mma.sync m16n8k32): q, scaled by a power of two per row, and the weights p, relative
-// to their own tile's maximum, are 23-bit integers X = x0 + 256 x1 + 65536 x2 with balanced int8 digits, so every digit
-// product is exact in int32 and a result is off only by the rounding of X (2^-22 of the row's largest |q|, 2^-23
-// of the tile's largest weight). A kv head serves at most 8 query heads at a time and the instruction has 16 rows: rows
-// 0-7 hold digit 0 and rows 8-15 digit 1, whose products then meet in one thread; a second instruction holds digit 2.
-// An accumulator starts at the bits of 1.5 * 2^23, so that read as fp32 it is its integer, without a conversion.
+// to their own tile's maximum, are 31-bit integers X = x0 + 2^8 x1 + 2^16 x2 + 2^24 x3 with balanced int8 digits, so
+// every digit product is exact in int32 and the rounding of X is at most 2^-30 of the row's largest |q|, or of the
+// tile's largest weight: below the 2^-24 of fp32 itself for all that is not 64 times smaller. A kv head serves at most 8
+// query heads at a time and the instruction has 16 rows: rows 0-7 hold digit 0 and rows 8-15 digit 1, whose products
+// then meet in one thread; a second instruction holds digits 2 and 3 (three digits of 23 bits took as many instructions,
+// 21.1 us where four take 21.5, and lost channels beside one that is 1000 times larger). An accumulator starts at the bits of 1.5 * 2^-6, whose last
+// place is 2^-29: read as fp32 it is its integer in units of X, without a conversion.
 // Each tile is joined to the running maximum and sums in fp32, so weights that are small beside another tile's keep
 // their bits.
 //
 // Bound: HBM bytes of the cache (256 + 8/64 per token and kv head). Measured on B200 (12 heads on 2): 64 sequences x 2048
-// 21.1 us (67.7 MB, 3.2 TB/s; loads alone 18.1, arithmetic alone 18.1, two warps per scheduler hide either only in
-// part), 1 x 131072 29.5 us, 1 x 517 10.1 us. On fp16 halves (m16n8k16) the codes' conversion cost 350 instructions per
+// 21.5 us (67.7 MB, 3.2 TB/s; loads alone 18.1, arithmetic alone 18.1, two warps per scheduler hide either only in
+// part), 1 x 131072 29.2 us, 1 x 517 10.7 us. On fp16 halves (m16n8k16) the codes' conversion cost 350 instructions per
 // tile where the digits cost 64, and 64 x 2048 took 27.5 us; tensor-map loads instead of cp.async gave 21.6.
 //
 // Split: all (row, kv head) items lie end to end as tiles, in equal runs over the CTAs and in each CTA over its warps,
@@ -106,8 +108,9 @@ __device__ __forceinline__ void mma(int (&d)[4], unsigned a0, unsigned a1, unsig
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-constexpr float kZero = 12582912.0f;  // 1.5 * 2^23: kZero + n for |n| < 2^22 has the bits of kZero plus n
-constexpr int kZeroBits = 0x4b400000;
+constexpr float kUnits = 536870912.0f;  // 2^29: X of 1
+constexpr float kZero = 1.5f / 64.0f;   // kZero + n / kUnits for |n| < 2^22 has the bits of kZero plus n
+constexpr int kZeroBits = 0x3cc00000;
 __device__ __forceinline__ void mma_first(int (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
                                           unsigned b1, const int (&zero)[4]) {
   asm volatile(
@@ -143,24 +146,29 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
   return r;
 }
 
-// Digits: the bytes of X + 0x808080 are the digits + 128, and flipping their top bits makes them int8. `x` is kZero + X,
-// whose low 24 bits are X + 0x400000.
-__device__ __forceinline__ unsigned digits(float x) { return (__float_as_uint(x) + 0x00408080u) ^ 0x00808080u; }
-// The digits of four numbers, regrouped by digit.
-__device__ __forceinline__ void by_digit(unsigned x0, unsigned x1, unsigned x2, unsigned x3, unsigned (&d)[3]) {
-  const unsigned a = __byte_perm(x0, x1, 0x5140), b = __byte_perm(x2, x3, 0x5140);
-  d[0] = __byte_perm(a, b, 0x5410);
-  d[1] = __byte_perm(a, b, 0x7632);
-  d[2] = __byte_perm(__byte_perm(x0, x1, 0x0062), __byte_perm(x2, x3, 0x0062), 0x5410);
+// Digits of x in [-2, 2]: the bytes of X + 0x808080 are the lower digits + 128 and the top one, and flipping the top bits of
+// the lower ones makes them int8.
+__device__ __forceinline__ unsigned digits(float x) {
+  return ((unsigned)__float2int_rn(x * kUnits) + 0x00808080u) ^ 0x00808080u;
 }
-// Two columns' digit sums to two fp32 numbers: lo is (digit 0, digit 1) of both, hi digit 2, each kZero off. The 256
-// folds digit 0's kZero into digit 1's difference; all steps are exact up to the last two roundings, of 2^-24 each.
+// 4 x 4 bytes transposed: byte i of the four words to word i. Of numbers to digits, of tokens to dims.
+__device__ __forceinline__ void transpose(unsigned x0, unsigned x1, unsigned x2, unsigned x3, unsigned (&d)[4]) {
+  const unsigned l0 = __byte_perm(x0, x1, 0x5140), h0 = __byte_perm(x0, x1, 0x7362);
+  const unsigned l1 = __byte_perm(x2, x3, 0x5140), h1 = __byte_perm(x2, x3, 0x7362);
+  d[0] = __byte_perm(l0, l1, 0x5410);
+  d[1] = __byte_perm(l0, l1, 0x7632);
+  d[2] = __byte_perm(h0, h1, 0x5410);
+  d[3] = __byte_perm(h0, h1, 0x7632);
+}
+// Two columns' digit sums to two fp32 numbers: lo is (digit 0, digit 1) of both, hi (digit 2, digit 3), each kZero off. The
+// 256 folds the lower digit's kZero into the upper one's difference, which stays exact; three roundings of 2^-24 follow.
 __device__ __forceinline__ u64 join_digits(const int (&lo)[4], const int (&hi)[4]) {
-  const u64 d0 = pair(__int_as_float(lo[0]), __int_as_float(lo[1])), d1 = pair(__int_as_float(lo[2]), __int_as_float(lo[3])),
-            d2 = pair(__int_as_float(hi[0]), __int_as_float(hi[1]));
   constexpr float kBoth = -(kZero + kZero / 256.0f);
-  const u64 y = fma2(add2(d1, pair(kBoth, kBoth)), pair(256.0f, 256.0f), d0);
-  return fma2(add2(d2, pair(-kZero, -kZero)), pair(65536.0f, 65536.0f), y);
+  auto join = [](const int(&d)[4]) {
+    return fma2(add2(pair(__int_as_float(d[2]), __int_as_float(d[3])), pair(kBoth, kBoth)), pair(256.0f, 256.0f),
+                pair(__int_as_float(d[0]), __int_as_float(d[1])));
+  };
+  return fma2(join(hi), pair(65536.0f, 65536.0f), join(lo));
 }
 
 __device__ __forceinline__ unsigned word(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
@@ -218,7 +226,7 @@ __device__ __forceinline__ void put_lse(const Attend& a, long long row, int h, f
 
 // This lane's dims of one query head as digits, and what a score of them is multiplied by.
 struct Query {
-  unsigned d[8][3];  // dims 32 q4 + 4 i + {0 .. 3} of head g
+  unsigned d[8][4];  // dims 32 q4 + 4 i + {0 .. 3} of head g
   float scale;       // scale * log2(e) * the power of two that was taken out
 };
 
@@ -401,17 +409,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
                            max(__float_as_uint(x[i].z) & 0x7fffffffu, __float_as_uint(x[i].w) & 0x7fffffffu)));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^21 and less of them, with the row's largest value in [2^21, 2^22) after the scaling; a NaN or an infinity in
-      // the row makes all its scores NaN
+      // the row's largest value is in [1, 2) after the scaling, in [0.5, 1) and doubled where 2^-127, which is no normal
+      // number, would be asked for; a NaN or an infinity in the row makes all its scores NaN
       const int e = top == 0 ? 127 : min(254, max(1, (int)(top >> 23)));
-      // the exponent of 2^-127 is none of a normal number: half of it goes into the unit
       const float down = __uint_as_float((unsigned)max(1, 254 - e) << 23), up = __uint_as_float((unsigned)e << 23);
-      const float unit = e == 254 ? 1048576.0f : 2097152.0f;
-      q.scale = top >= 0x7f800000u ? __int_as_float(0x7fc00000) : a.scale * up * (1.4426950408889634f / 2097152.0f);
+      const float half = e == 254 ? 0.5f : 1.0f;
+      q.scale = top >= 0x7f800000u ? __int_as_float(0x7fc00000) : up * 1.4426950408889634f * a.scale;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        by_digit(digits(fmaf(x[i].x * down, unit, kZero)), digits(fmaf(x[i].y * down, unit, kZero)),
-                 digits(fmaf(x[i].z * down, unit, kZero)), digits(fmaf(x[i].w * down, unit, kZero)), q.d[i]);
+        transpose(digits(x[i].x * down * half), digits(x[i].y * down * half), digits(x[i].z * down * half),
+                  digits(x[i].w * down * half), q.d[i]);
     };
 
     int it_row = row, it_sub = sub;
@@ -454,16 +461,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
           b[j] = *reinterpret_cast<const uint4*>(kt + (j * 8 + g) * kHead + (((q4 * 2 + h) ^ g) << 4));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const unsigned(&x)[3] = q.d[h * 4 + i * 2], (&y)[3] = q.d[h * 4 + i * 2 + 1];
+          const unsigned(&x)[4] = q.d[h * 4 + i * 2], (&y)[4] = q.d[h * 4 + i * 2 + 1];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const unsigned b0 = i ? b[j].z : b[j].x, b1 = i ? b[j].w : b[j].y;
             if (h == 0 && i == 0) {
               mma_first(lo[j], x[0], x[1], y[0], y[1], b0, b1, zero);
-              mma_first(hi[j], x[2], 0, y[2], 0, b0, b1, zero);
+              mma_first(hi[j], x[2], x[3], y[2], y[3], b0, b1, zero);
             } else {
               mma(lo[j], x[0], x[1], y[0], y[1], b0, b1);
-              mma(hi[j], x[2], 0, y[2], 0, b0, b1);
+              mma(hi[j], x[2], x[3], y[2], y[3], b0, b1);
             }
           }
         }
@@ -494,17 +501,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
         for (int i = 0; i < 2; ++i) p[j][i] = ex2(p[j][i] - tm);
         tl += p[j][0] + p[j][1];
       }
-      const float mn = fmaxf(m, tm), keep = ex2(m - mn), add = ex2(tm - mn), av = add * (vs * (1.0f / 4194304.0f));
+      const float mn = fmaxf(m, tm), keep = ex2(m - mn), add = ex2(tm - mn), av = add * vs;
       m = mn;
       l = l * keep + add * tl;
       const unsigned long long keep2 = pair(keep, keep), av2 = pair(av, av);
 
-      // this lane's weights are what it holds of the operand: 2^22 and less
-      unsigned pd[2][3];
+      // this lane's weights are what it holds of the operand
+      unsigned pd[2][4];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        by_digit(digits(fmaf(p[2 * k][0], 4194304.0f, kZero)), digits(fmaf(p[2 * k][1], 4194304.0f, kZero)),
-                 digits(fmaf(p[2 * k + 1][0], 4194304.0f, kZero)), digits(fmaf(p[2 * k + 1][1], 4194304.0f, kZero)), pd[k]);
+        transpose(digits(p[2 * k][0]), digits(p[2 * k][1]), digits(p[2 * k + 1][0]), digits(p[2 * k + 1][1]), pd[k]);
       uint4 raw[2][4];  // dims 16 g .. 16 g + 15 of tokens 16 k + 2 q4 + {0, 1, 8, 9}
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -515,23 +521,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
         }
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        // 4 x 4 bytes: from four dims of a token to four tokens of a dim
-        unsigned b[2][4];
+        unsigned b[2][4];  // from four dims of a token to four tokens of a dim
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const unsigned x0 = word(raw[k][0], w), x1 = word(raw[k][1], w), x2 = word(raw[k][2], w), x3 = word(raw[k][3], w);
-          const unsigned l0 = __byte_perm(x0, x1, 0x5140), h0 = __byte_perm(x0, x1, 0x7362);
-          const unsigned l1 = __byte_perm(x2, x3, 0x5140), h1 = __byte_perm(x2, x3, 0x7362);
-          b[k][0] = __byte_perm(l0, l1, 0x5410);
-          b[k][1] = __byte_perm(l0, l1, 0x7632);
-          b[k][2] = __byte_perm(h0, h1, 0x5410);
-          b[k][3] = __byte_perm(h0, h1, 0x7632);
-        }
+        for (int k = 0; k < 2; ++k)
+          transpose(word(raw[k][0], w), word(raw[k][1], w), word(raw[k][2], w), word(raw[k][3], w), b[k]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           int dl[4], dh[4];
           mma_first(dl, pd[0][0], pd[0][1], pd[1][0], pd[1][1], b[0][i], b[1][i], zero);
-          mma_first(dh, pd[0][2], 0, pd[1][2], 0, b[0][i], b[1][i], zero);
+          mma_first(dh, pd[0][2], pd[0][3], pd[1][2], pd[1][3], b[0][i], b[1][i], zero);
           o[w * 4 + i] = fma2(av2, join_digits(dl, dh), mul2(o[w * 4 + i], keep2));
         }
       }
