@@ -744,3 +744,21 @@ def test_attention_small_weights_beside_a_large_one(below):
         tol = 2.0**-30 * (1 + 2.0**-6) * np.abs(v).sum(0) / p.sum() + (2 * d + 52 * u) * (p @ np.abs(v)) / p.sum() + 2.0**-149
         assert (np.abs(got[h] - want) <= tol).all(), (h, np.abs(got[h] - want).max(), tol.min())
         assert abs(float(lse[0, h]) - (s.max() + np.log(p.sum()))) <= 2 * d + 52 * u
+
+
+@pytest.mark.parametrize("size", [1e-37, 1e-30, 1e-20, 1e20, 1e34])
+def test_attention_sizes_of_values(size):
+    """Values of V far from 1, down to scales of a few smallest normal numbers: the result keeps all of their bits."""
+    import torch
+
+    u, n = 2.0**-24, 150
+    c = filled([n], 2, seed=25)
+    c.model["v"].scales[:] = np.float32(size)
+    c.scales["v"].copy_(torch.as_tensor(c.model["v"].scales))
+    q = torch.randn(1, 12, 128, generator=torch.Generator().manual_seed(5)).cuda()
+    out, lse, _ = attend(c, q, "f32", ints([0]), ints([n]))
+    k, v = (values64(c, w, 0, n) for w in "kv")
+    want, _, mag = km.attention(q[0].cpu().numpy(), k, v, float(np.float32(SCALE)))
+    # scores: 12 roundings of a sum of absolute products; 2 d of them, weights and sums of 5 tiles
+    eps = 2 * 12 * u * mag + 2.0**-29 + 100 * u
+    assert (np.abs(out[0].cpu().numpy() - want) <= eps * np.abs(v).max() + 2.0**-149).all()
