@@ -523,3 +523,22 @@ def test_engine_keeps_no_logits_of_steps_that_were_not_asked_for():
         assert list(eng.sample([0.5, 0.5], temperature=[0.0, 0.0])[0]) == list(eng.read_logits(2).argmax(1))
     finally:
         eng.close()
+
+
+def test_engine_rows_that_leave_settings_open():
+    from work_llm_accelerator_b200 import host
+
+    eng = host.Engine(0, 8, max_seqs=3, max_len=64)
+    try:
+        eng.init_synthetic(5)
+        eng.set_option("logits", 1)
+        for slot in range(3):
+            eng.prefill(slot, [slot + 1, 7])
+        eng.decode([0, 1, 2], [3, 3, 3])
+        u = [0.9, 0.8, 0.999]
+        want = eng.sample(u, temperature=[1.0, 0.0, 0.5], top_k=[0, 5, 9], top_p=[1.0, 1.0, 0.9], min_p=[0.1, 0.0, 0.0])
+        got = eng.sample(u, temperature=[None, 0.0, 0.5], top_k=[None, 5, 9], top_p=[None, None, 0.9], min_p=[0.1, None, None])
+        np.testing.assert_array_equal(got[0], want[0])
+        np.testing.assert_array_equal(got[1], want[1])
+    finally:
+        eng.close()

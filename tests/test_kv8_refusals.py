@@ -133,3 +133,11 @@ def test_model_sampler():
     assert list(km.kept(x, min_p=0.3)[0]) == [1, 3, 2] and list(km.kept(x, min_p=0.4)[0]) == [1, 3]
     assert km.sample(x, 0.0)[0] == 1 and km.sample(x, 0.999)[0] == 0
     assert km.sample([-np.inf, np.nan], 0.5) == (-1, 0.0)
+
+
+def test_rows_that_leave_a_setting_open(host):
+    """None in a row: the value that turns the filter off, temperature 1 (a NaN would mean greedy)."""
+    assert host._per_row(None, 1.0, np.float32) is None
+    np.testing.assert_array_equal(host._per_row([None, 0.5, 0.0], 1.0, np.float32), np.float32([1.0, 0.5, 0.0]))
+    np.testing.assert_array_equal(host._per_row((7, None), 0, np.int32), np.int32([7, 0]))
+    np.testing.assert_array_equal(host._per_row(np.float32([0.25, 0.5]), 0.0, np.float32), np.float32([0.25, 0.5]))

@@ -249,6 +249,11 @@ def _check(status: int, what: str) -> None:
         raise EngineError(f"{what} failed with status {status} ({STATUS_TEXT.get(status, '?')}): {last_error()}")
 
 
+def _per_row(values: Sequence | None, off: float, dtype) -> np.ndarray | None:
+    """A setting's array with `off` in the rows that leave it open; None where all do."""
+    return None if values is None else np.array([off if v is None else v for v in values], dtype)
+
+
 class Engine:
     """Device-resident 28-layer engine on one GPU (include/qwen_b200_engine.h)."""
 
@@ -356,14 +361,14 @@ class Engine:
         _check(self.lib.qwen_engine_read_logits(self.handle, out, out.size), "read_logits")
         return out.reshape(rows, VOCAB)
 
-    def sample(self, uniforms: Sequence[float], temperature: Sequence[float] | None = None,
-               top_k: Sequence[int] | None = None, top_p: Sequence[float] | None = None,
-               min_p: Sequence[float] | None = None) -> tuple[np.ndarray, np.ndarray]:
+    def sample(self, uniforms: Sequence[float], temperature: Sequence[float | None] | None = None,
+               top_k: Sequence[int | None] | None = None, top_p: Sequence[float | None] | None = None,
+               min_p: Sequence[float | None] | None = None) -> tuple[np.ndarray, np.ndarray]:
         """(tokens, probabilities) sampled from the last call's logits, a row per uniform number (option "logits" on;
-        include/qwen_b200_engine.h). Settings are per row, None: off."""
+        include/qwen_b200_engine.h). Settings are per row; None, for one row or for all: temperature 1, the others off."""
         u = np.ascontiguousarray(uniforms, np.float32)
-        rows = [None if v is None else np.ascontiguousarray(v, t)
-                for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        rows = [_per_row(temperature, 1.0, np.float32), _per_row(top_k, 0, np.int32), _per_row(top_p, 1.0, np.float32),
+                _per_row(min_p, 0.0, np.float32)]
         if any(v is not None and v.shape != u.shape for v in rows) or u.ndim != 1:
             raise ValueError("sample: one setting per uniform number")
         tokens, probs = np.zeros(u.size, np.int32), np.zeros(u.size, np.float32)
