@@ -145,6 +145,8 @@ int qwen_b200_kv8_read(const qwen_b200_kv8_cache* cache, void* k, void* v, int d
  * Both products are sums of integers: a query head is held to 2^-30 of its largest channel, and a weight to 2^-30 of the
  * largest of the up to 32 tokens that it is computed with, in place of 2^-24 of itself; the sums are exact, and what
  * follows is fp32.
+ * A call repeats bit for bit. How a row's tokens are split into parts follows from the lengths of all rows, so the same row
+ * in another batch, or at another place, may differ by the roundings of its sums.
  * row_lens[r] == 0: out is 0 and lse -infinity. row_seqs[r] < 0 (a padded row): out and lse are left as they are.
  *   q, out     [n_rows] rows of n_q_heads x 128 values of `dtype` (16-byte aligned, strides in elements, multiples
  *              of 16 bytes); out must not overlap q

@@ -762,3 +762,22 @@ def test_attention_sizes_of_values(size):
     # scores: 12 roundings of a sum of absolute products; 2 d of them, weights and sums of 5 tiles
     eps = 2 * 12 * u * mag + 2.0**-29 + 100 * u
     assert (np.abs(out[0].cpu().numpy() - want) <= eps * np.abs(v).max() + 2.0**-149).all()
+
+
+def test_attention_rows_in_another_order_or_batch():
+    """The same rows permuted, and a few of them alone: other splits of the work, so equal up to the bound of check_rows, and
+    each order repeats bit for bit."""
+    import torch
+
+    lens = [3000, 17, 900, 0, 2222, 64, 5000]
+    n = len(lens)
+    c = filled(lens, 2, seed=32)
+    q = torch.randn(n, 12, 128, generator=torch.Generator().manual_seed(8)).cuda()
+    r = np.random.RandomState(4)
+    for order in [list(range(n)), list(range(n))[::-1], list(r.permutation(n)), [4], [6, 2], [2, 6]]:
+        ns = [lens[i] for i in order]
+        out, lse, _ = attend(c, q[order], "f32", ints(order), ints(ns))
+        again, lse2, _ = attend(c, q[order], "f32", ints(order), ints(ns))
+        torch.cuda.synchronize()
+        check_rows(c, q[order], "f32", order, ns, out, lse)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
