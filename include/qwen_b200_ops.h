@@ -168,13 +168,14 @@ long long qwen_b200_kv8_attention_workspace(int n_rows, int n_q_heads, int n_kv_
  *   top_p < 1  keeps the fewest of those, at least one, whose sum of w reaches top_p of their whole sum;
  *   min_p > 0  keeps those of w >= min_p (the first one in any case);
  * the token is the first whose running sum of w exceeds uniform * (sum of the kept w), the last one kept if none does.
- * temperature below 2^-126 (0 included) or NaN: the first token, with probability 1. Logits of -infinity or NaN are
+ * temperature below 2^-126 (0 included) or NaN: the first token, with probability 1; one from there to 2^-121 counts as
+ * 2^-121. Logits of -infinity or NaN are
  * never taken; a row without any other gives token -1, probability 0. +infinity outweighs every finite logit. Weights
  * below exp(-32) of the largest count as 0; the others are within (2 + z) 2^-24 of themselves, z = (max - logit) /
- * temperature.
+ * temperature; a logit whose distance from the largest is beyond the fp32 range counts as -infinity.
  *   logits      [rows][vocab] of `dtype`, rows row_stride elements apart; 1 <= vocab <= 262144
  *   temperature, top_k, top_p, min_p  [rows] fp32 / int32, or NULL (1, off, off, off)
- *   uniforms    [rows] fp32 in [0, 1)
+ *   uniforms    [rows] fp32 in [0, 1); below (or NaN) counts as 0, above draws the last token kept
  *   tokens      [rows] int32;  probs  [rows] fp32: the probability that the token had among the kept ones, or NULL
  * All device memory. The result does not depend on the order in which anything is summed on the GPU. */
 int qwen_b200_sample(const void* logits, int dtype, int rows, int vocab, long long row_stride, const float* temperature,

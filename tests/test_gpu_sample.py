@@ -542,3 +542,20 @@ def test_engine_rows_that_leave_settings_open():
         np.testing.assert_array_equal(got[1], want[1])
     finally:
         eng.close()
+
+
+@pytest.mark.parametrize("t,acts", [(2.0**-126, 2.0**-121), (1.5 * 2.0**-124, 2.0**-121), (2.0**-121, 2.0**-121), (1.3 * 2.0**-119, 1.3 * 2.0**-119)])
+def test_the_smallest_temperatures(t, acts):
+    """Logits as close to one another as the smallest temperatures are to 0: from 2^-126 to 2^-121 they act as 2^-121."""
+    import torch
+
+    step = 2.0**-121
+    x = torch.tensor([[3 * step, 0.0, 1.5 * step, 3 * step]])
+    ids, w = km.kept(x[0].numpy(), acts)
+    for kw in ({}, {"min_p": [0.1]}):
+        n = 4 if not kw else int((w >= 0.1).sum())
+        p = w[:n] / w[:n].sum()
+        for at in range(n):
+            got, prob = run(x, [float(np.cumsum(p)[at] - p[at] / 2)], temperature=[t], **kw)
+            assert got[0] == ids[at], (at, kw)
+            np.testing.assert_allclose(prob, p[at], rtol=2.0**-18)

@@ -115,7 +115,7 @@ struct Scale {
     const float r = 1.0f / t;
     float low = r > 0.0f ? fmaf(-t, r, 1.0f) * r : 0.0f;
     if (!(fabsf(low) < r)) low = 0.0f;
-    c = fminf(64.0f * r, 3.4028235e38f);  // finite, so that the best token stays at 0 steps
+    c = 64.0f * r;
     c_low = 64.0f * low;
   }
   static constexpr float kFloor = 8388608.0f;  // 2^23: added rounding down, the sum's low bits are the floor
@@ -819,8 +819,8 @@ __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kCl == k
     return;
   }
   r.top_infinite = value_of(best) == INFINITY;
-  r.scale = Scale(r.seen(value_of(best)), t);
-  r.temperature = t;
+  r.temperature = fmaxf(t, 3.7615819e-37f);  // 2^-121: 64 / t stays finite, so that the best token stays at 0 steps
+  r.scale = Scale(r.seen(value_of(best)), r.temperature);
   r.least = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   r.template add_up<false>({kHistogram, 0, kBuckets - 1, 0, 0, 0, {}, {}});
   r.share_sums();
