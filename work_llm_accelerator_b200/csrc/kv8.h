@@ -43,7 +43,7 @@ struct Attend {
   float scale;
   void* work;
 };
-size_t attention_workspace(int rows, int q_heads, int heads);
+size_t attention_workspace(int rows, int q_heads, int heads);  // the same for all: it follows from the number of CTAs
 cudaError_t launch_attention(const Cache& c, const Attend& a, int type, cudaStream_t s);
 
 // Error flags of the kernels on the current device (kErrMbarTimeout, kErrBadIndex).

@@ -15,9 +15,11 @@
 // their bits.
 //
 // Bound: HBM bytes of the cache (256 + 8/64 per token and kv head). Measured on B200 (12 heads on 2): 64 sequences x 2048
-// 21.5 us (67.7 MB, 3.2 TB/s; loads alone 18.1, arithmetic alone 18.1, two warps per scheduler hide either only in
-// part), 1 x 131072 29.2 us, 1 x 517 10.7 us. On fp16 halves (m16n8k16) the codes' conversion cost 350 instructions per
-// tile where the digits cost 64, and 64 x 2048 took 27.5 us; tensor-map loads instead of cp.async gave 21.6.
+// 21.5 us (67.7 MB), of which the loop over the tiles takes 11, near the rate of HBM; the rest does not grow with the
+// lengths: schedule 2.4, query and first tiles 2.7, join of the warps 1.9, launch. 1 x 131072 29.2 us (loop 15, join of
+// the CTAs' parts 6), 1 x 517 10.7 us. On fp16 halves (m16n8k16) the codes' conversion cost 350 instructions per tile
+// where three digits cost 64, and 64 x 2048 took 27.5 us (1 x 131072 26.8); tensor-map loads instead of cp.async took
+// 0.5 us more.
 //
 // Split: all (row, kv head) items lie end to end as tiles, in equal runs over the CTAs and in each CTA over its warps,
 // whatever the lengths are; a border that would cut an item moves to its beginning where that makes no run much longer.
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(Cache c, Attend 
   }
 }
 
-// A number that no earlier call had, in the upper 48 bits.
+// A number for a call, in the upper 48 bits: a counter through the finaliser of splitmix64 (Steele, Lea and Flood, 2014).
 u64 call_number() {
   static std::atomic<u64> next{(u64)std::chrono::steady_clock::now().time_since_epoch().count()};
   u64 x = next.fetch_add(0x9e3779b97f4a7c15ull);

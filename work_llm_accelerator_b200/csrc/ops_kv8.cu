@@ -131,7 +131,6 @@ int rows_call(const char* op, const qwen_b200_kv8_cache* c, const void* k, const
               long long n_rows, const int* seqs, const int* starts, const int* offsets, int n_segments, void* stream) {
   if (!cache_ok(op, c) || !range_ok(op, "dtype", dtype, QWEN_B200_F32, QWEN_B200_BF16) ||
       !range_ok(op, "n_rows", n_rows, 0, kMaxRows) || !range_ok(op, "n_segments", n_segments, 0, kMaxRows) ||
-      !range_ok(op, "n_kv_heads", c->n_kv_heads, 1, 1024) ||
       !stride_ok(op, "row_stride", row_stride, (long long)c->n_kv_heads * kv8::kHead, dtype))
     return kStatusInvalid;
   if (n_rows == 0 || n_segments == 0) return 0;

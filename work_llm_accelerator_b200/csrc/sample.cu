@@ -18,8 +18,9 @@
 // once, two per SM. The first CTA leads: it gets the others' bucket sums through distributed shared memory, decides (every
 // warp the same way, without barriers) and asks for what it needs to see. Bound: for few rows
 // the latency of those steps, for many the two shared atomics per logit of the second pass (4.1 cycles each at random
-// banks). Measured on B200, vocabulary 151936: 1 fp32 row with all filters 18.2 us, 64 rows with settings of their own 64
-// us, 256 bf16 rows without filters 119 us.
+// banks). Measured on B200, vocabulary 151936: 1 fp32 row with all filters 19.0 us, 64 rows with settings of their own
+// 65.3 us, 256 bf16 rows without filters 120 us. Two CTAs per SM leave 64 registers, of which the leader's part spills
+// 0.6 to 1 KB; with 128 and one CTA per SM 64 rows take 78 us and 256 rows 124 (but 150 rows 114 instead of 139).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -119,8 +120,8 @@ struct Scale {
     c_low = 64.0f * low;
   }
   static constexpr float kFloor = 8388608.0f;  // 2^23: added rounding down, the sum's low bits are the floor
-  // q + kQBits as bits: the conversion is the addition of 1.5 * 2^23. The 64 keeps a q of -12 positive, which the
-  // rounding of a step count next to its bucket's border can give.
+  // q + kQBits as bits: the conversion is the addition of 1.5 * 2^23. The 64 keeps a q of -24 positive: next to a bucket's
+  // border near 2048 a step count can round up by 2^-14 (8 of q) and c_low add a lack of 2^-13 (16).
   static constexpr float kRound = 12582912.0f + 64.0f;
   static constexpr unsigned kQBits = 0x4b400000u + 64u;
   // 2^23 (1 - exp(-f / 64)) = k1 f + k2 f^2 + k3 f^3 + k4 f^4, the next term below 2^-36 of it
@@ -766,7 +767,7 @@ struct Row {
   }
 };
 
-// A cluster of 8 has its SMs to itself and takes the registers that the leader's part wants (1 row: 18.3 us, 20.9 with 64).
+// A cluster of 8 has its SMs to itself and takes the registers that the leader's part wants (1 row: 19.2 us, 21.5 with 64).
 template <int kType, int kCl>
 __global__ void __cluster_dims__(kCl, 1, 1) __launch_bounds__(kThreads, kCl == kMaxCluster ? 1 : 2)
     sample_kernel(Sample a, int slice) {
