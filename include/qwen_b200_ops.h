@@ -131,7 +131,8 @@ int qwen_b200_kv8_append(const qwen_b200_kv8_cache* cache, const void* k, const 
                          const int* offsets, int n_segments, void* stream);
 
 /* Read cached rows back: segment i writes tokens starts[i] .. of sequence seqs[i] to rows offsets[i] ..
- * offsets[i + 1] - 1 of k and v (different buffers), as code * scale rounded to `dtype`. Arguments as above; rows from
+ * offsets[i + 1] - 1 of k and v (different buffers), as code * scale rounded to `dtype` (a value within 1% of the
+ * type's largest number can lie beyond it by then, and reads as infinity). Arguments as above; rows from
  * offsets[n_segments] on are left as they are, and a sequence may be named more than once. */
 int qwen_b200_kv8_read(const qwen_b200_kv8_cache* cache, void* k, void* v, int dtype, long long row_stride,
                        long long n_rows, const int* seqs, const int* starts, const int* offsets, int n_segments,

@@ -781,3 +781,22 @@ def test_attention_rows_in_another_order_or_batch():
         torch.cuda.synchronize()
         check_rows(c, q[order], "f32", order, ns, out, lse)
         assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_read_next_to_the_largest_number():
+    """65504 in a block whose scale was doubled is a number of steps rounded up: documented to read as infinity in fp16;
+    within a step in fp32."""
+    c = Cache([2], 1, seed=26)
+    c.append({w: np.full((1, 1, 128), 35000.0, np.float32) for w in "kv"}, "f32", [0], [0], [1])
+    c.append({w: np.full((1, 1, 128), 65504.0, np.float32) for w in "kv"}, "f16", [0], [1], [1])
+    c.check([2])
+    for dtype in ("f16", "f32"):
+        out, _ = c.read(dtype, [0], [0], [2])
+        for w in "kv":
+            want = c.model[w].values(0, 2)
+            with np.errstate(over="ignore"):
+                want = want.astype(np.float16).astype(np.float32) if dtype == "f16" else want
+            np.testing.assert_array_equal(out[w].float().cpu().numpy(), want)
+            if dtype == "f32":
+                step = c.model[w].scales[c.table[0, 0]][0]
+                assert (np.abs(want[:, 0] - [[35000.0], [65504.0]]) < step).all()
