@@ -9,8 +9,8 @@
 // tile's largest weight: below the 2^-24 of fp32 itself for all that is not 64 times smaller. A kv head serves at most 8
 // query heads at a time and the instruction has 16 rows: rows 0-7 hold digit 0 and rows 8-15 digit 1, whose products
 // then meet in one thread; a second instruction holds digits 2 and 3 (three digits of 23 bits took as many instructions,
-// 21.1 us where four take 21.5, and lost channels beside one that is 1000 times larger). An accumulator starts at the bits of 1.5 * 2^-6, whose last
-// place is 2^-29: read as fp32 it is its integer in units of X, without a conversion.
+// 21.1 us where four take 21.5, and lost channels beside one that is 1000 times larger). An accumulator starts at the
+// bits of 1.5 * 2^-6, whose last place is 2^-29: read as fp32 it is its integer in units of X, without a conversion.
 // Each tile is joined to the running maximum and sums in fp32, so weights that are small beside another tile's keep
 // their bits.
 //
